@@ -49,6 +49,12 @@ extern "C" {
 #define QVX_F32 0
 #define QVX_BF16 1
 #define QVX_F16 2
+/* 4 bits: groups of 32 elements of a row share an f16 step s >= 0 and an f16 offset z, and code c (0..15) stands for
+ * z + s c: 5 bits an element (the numerics of GGUF's Q4_1).  z is the group's least value rounded down, s is
+ * (greatest - z) / 15 rounded up, so a stored element is off by at most s / 2; a group with a NaN, an infinity or a value
+ * beyond 65504 stands for NaN.  Pools only, native layout only: block_tokens a multiple of 16, head_dim 64, 128 or 256;
+ * rows go in and come out as f32 (or 16-bit, qvx_kv_read). */
+#define QVX_Q4 3
 
 /* The reference's block: keys [kv_head][d][B] then values [B][kv_head][d]
  * (crates/qubivex-compute/src/discrete.rs:247-256, :317-329), B generalised from 256. */
@@ -57,6 +63,10 @@ extern "C" {
  * One position's row is contiguous (16-byte stores), one (block, kv head) page pair is
  * contiguous (one bulk copy).  Needs head_dim * element size to be a multiple of 128. */
 #define QVX_LAYOUT_NATIVE 1
+
+/* In place of a position in device memory: no token here (the padding of a batch).  qvx_kv_append, qvx_kv_sync,
+ * qvx_kv_read and qvx_head_prelude pass over such a row, qvx_attn_decode_window writes zeros for it. */
+#define QVX_POS_NONE 0xffffffffu
 
 typedef struct qvx_geometry {
     uint32_t block_tokens; /* KV_BLOCK, discrete.rs:248 */
@@ -69,7 +79,8 @@ typedef struct qvx_geometry {
 /* kv_block_words x element size (discrete.rs:253-256).  0 for a geometry that is not valid. */
 size_t qvx_block_bytes(const qvx_geometry *geo);
 /* Byte offset in the pool of key (kv = 0) or value (kv = 1) element (g, i) at pool position
- * `at` = block * block_tokens + slot: kv_key_word / kv_value_word (discrete.rs:317-329). */
+ * `at` = block * block_tokens + slot: kv_key_word / kv_value_word (discrete.rs:317-329).  Of a 4-bit pool: the byte
+ * the element's code lies in. */
 size_t qvx_elem_offset(const qvx_geometry *geo, size_t at, int kv, size_t g, size_t i);
 
 /* ---- the device (trait DiscreteDevice, crates/qubivex-compute/src/discrete.rs:433-570) -- */
@@ -157,6 +168,14 @@ int32_t qvx_kv_append(qvx_device *dev, const qvx_geometry *geo, void *pool, size
                       const float *k_new, const float *v_new, const uint32_t *pos,
                       const uint32_t *blocks, const uint32_t *table_at, size_t s, void *stream);
 
+/* Rows as the pool holds them: row r of `rows` (n x 2*kv_out of rows_dtype QVX_F32, QVX_BF16 or QVX_F16, rounded to
+ * nearest: key row, value row) becomes what pool position from[r] = block * block_tokens + slot stands for.  The reverse
+ * of qvx_kv_sync, for any pool: what a host cache, another pool or a prompt's attention takes back from a 4-bit or 16-bit
+ * cache.  No counterpart in the reference, whose host cache holds every row.  A row whose block is at or past
+ * pool_blocks is left as it was (device status, as above). */
+int32_t qvx_kv_read(qvx_device *dev, const qvx_geometry *geo, const void *pool, size_t pool_blocks,
+                    const uint32_t *from, size_t n, void *rows, uint32_t rows_dtype, void *stream);
+
 /* Block tables of one decode op, resident on the device with the work list the split
  * kernel walks.  Built from host arrays, as DeviceMoeAttention carries them
  * (discrete.rs:292-297); validated as sim.rs:313-324, :359-376 does. */
@@ -242,6 +261,51 @@ typedef struct qvx_prelude {
  * take, and k_new / v_new what the host cache keeps (attn_prelude.comp's binding 2). */
 int32_t qvx_attn_prelude(qvx_device *dev, const qvx_geometry *geo, size_t heads, size_t s, float *q,
                          float *k_new, float *v_new, const qvx_prelude *prelude, void *stream);
+
+/* Decode attention over what a window and a few first positions leave visible: token t sees the positions
+ * j <= pos[t] of its own table with j < sinks or j > pos[t] - window; window 0: all of them.  No counterpart in the
+ * reference, which attends over everything.  Native-layout pools of every element type, head_dim 64, 128 or 256,
+ * block_tokens a multiple of 16.  pos, blocks and table_at are device arrays of s, n_blocks and s entries, read when the
+ * kernel runs: no tables object, no scratch, nothing kept between calls, so a captured launch can be replayed on changed
+ * positions and tables, and launches on different streams do not disturb each other.
+ * max_pos: a bound on pos[] the host knows (at most 0x7fffffff); it and the window choose how many CTAs share a token, so
+ * a token's bits depend on them, never on the rest of the batch.  A token beyond max_pos gets no output row (device
+ * status); one with QVX_POS_NONE gets zeros.  A table entry past n_blocks, or a block id at or past pool_blocks, is not
+ * read: its positions count as not visible and the device status says so.  What lies in slots that are not visible does
+ * not matter, NaN included.  Keys, values and queries that are seen are taken to be finite: an infinity among them may
+ * come out as NaN.  pool, q and out 16-byte aligned, else QVX_ERR_SHAPE.  s at most 65535. */
+int32_t qvx_attn_decode_window(qvx_device *dev, const qvx_geometry *geo, const void *pool, size_t pool_blocks,
+                               size_t heads, size_t s, const float *q, const uint32_t *pos, const uint32_t *blocks,
+                               size_t n_blocks, const uint32_t *table_at, uint32_t max_pos, uint32_t window,
+                               uint32_t sinks, float *out, void *stream);
+
+/* The prelude of decoders that norm each head by itself (qvx_attn_prelude norms the full width): RMS norm of every
+ * query and key head with one set of head_dim weights, NeoX RoPE on its first rot_dim elements (pairs (i, i + rot_dim/2))
+ * by row pos[t] of a table of [cos.., sin..] rows, values untouched, and, when a pool is given, the store of the key and
+ * value rows at pos[t] of the token's table (qvx_kv_append's place) -- one pass over the projections, which may be strided
+ * slices of one fused projection, f32, bf16 or f16.  Arithmetic in f32; not the reference's summation order.
+ * A token with QVX_POS_NONE is passed over; one at or past rope_rows is too, and the device status says so; a table entry
+ * past n_blocks or a block id at or past pool_blocks is not stored to (device status).  Outputs and pool 16-byte
+ * aligned, head_dim a multiple of 4.  q_out / k_out / v_out may be the inputs themselves where those are f32 and
+ * contiguous; otherwise inputs and outputs must not overlap. */
+typedef struct qvx_head_prelude {
+    const void *q, *k, *v;                 /* element (t, h, i) at t * stride + h * head_dim + i; `dtype` elements      */
+    uint64_t q_stride, k_stride, v_stride; /* elements from one token to the next                                   */
+    uint32_t dtype;                        /* QVX_F32, QVX_BF16 or QVX_F16                                          */
+    uint32_t rot_dim;                      /* even, <= head_dim; unused without `rope`                              */
+    const float *q_norm, *k_norm;          /* head_dim weights each; both NULL: no norms                            */
+    double eps;                            /* narrowed to f32 before use                                            */
+    const float *rope;                     /* rope_rows x rot_dim; NULL: no rotation                                */
+    uint32_t rope_rows;
+    const uint32_t *pos;                   /* s positions                                                           */
+    float *q_out;                          /* s x heads x head_dim                                                  */
+    float *k_out, *v_out;                  /* s x kv_heads x head_dim each; NULL: not wanted                        */
+    void *pool;                            /* NULL: nothing is stored                                               */
+    size_t pool_blocks, n_blocks;
+    const uint32_t *blocks, *table_at;     /* as qvx_kv_append's                                                    */
+} qvx_head_prelude;
+int32_t qvx_head_prelude_store(qvx_device *dev, const qvx_geometry *geo, size_t heads, size_t s,
+                               const qvx_head_prelude *prelude, void *stream);
 
 /* Whole-block copies src[i] -> dst[i]: the copy of a shared block before the first
  * divergent append, and the moves of a compaction pass.  No counterpart in the reference,

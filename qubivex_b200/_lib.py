@@ -32,6 +32,15 @@ class Prelude(C.Structure):
                 ("eps", C.c_double), ("rope", C.c_void_p)]
 
 
+class HeadPrelude(C.Structure):
+    """qvx_head_prelude."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("v_stride", C.c_uint64), ("dtype", C.c_uint32), ("rot_dim", C.c_uint32), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("eps", C.c_double), ("rope", C.c_void_p), ("rope_rows", C.c_uint32), ("pos", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("pool", C.c_void_p), ("pool_blocks", C.c_size_t), ("n_blocks", C.c_size_t),
+                ("blocks", C.c_void_p), ("table_at", C.c_void_p)]
+
+
 class Usage(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("capacity", "used", "peak", "refused")]
 
@@ -92,6 +101,10 @@ PROTOTYPES = {
     "qvx_reset_kernel_times": (C.c_int32, [P]),
     "qvx_kv_sync": (C.c_int32, [P, _GEO, P, C.c_size_t, P, P, C.c_size_t, P]),
     "qvx_kv_append": (C.c_int32, [P, _GEO, P, C.c_size_t, P, P, P, P, P, C.c_size_t, P]),
+    "qvx_kv_read": (C.c_int32, [P, _GEO, P, C.c_size_t, P, C.c_size_t, P, C.c_uint32, P]),
+    "qvx_attn_decode_window": (C.c_int32, [P, _GEO, P, C.c_size_t, C.c_size_t, C.c_size_t, P, P, P, C.c_size_t, P, C.c_uint32,
+                                           C.c_uint32, C.c_uint32, P, P]),
+    "qvx_head_prelude_store": (C.c_int32, [P, _GEO, C.c_size_t, C.c_size_t, C.POINTER(HeadPrelude), P]),
     "qvx_tables_create": (C.c_int32, [P, _GEO, C.c_size_t, C.c_size_t, C.c_size_t, P, P, C.c_size_t, P, C.POINTER(P)]),
     "qvx_tables_free": (None, [P]),
     "qvx_tables_pos": (P, [P]),

@@ -36,6 +36,9 @@ COMMON = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler",
 SOURCES = {
     "qvx_api.cu": [],
     "kv_rows.cu": [],
+    "kv_q4.cu": [],
+    "head_prelude.cu": [],
+    "attn_window.cu": [],
     "block_copy.cu": [],
     "attn_stream.cu": [],
     "attn_static.cu": [],

@@ -231,7 +231,7 @@ extern "C" int32_t qvx_attn_decode_static(qvx_device* dev, const qvx_geometry* g
     if (!geometry_ok(geo)) return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no KV pool of this geometry");
     std::lock_guard<std::mutex> lk(dev->mu);
     const Layout L = make_layout(geo);
-    if (L.layout != QVX_LAYOUT_NATIVE || L.dtype == QVX_F32 || (L.d != 64 && L.d != 128) || L.B % TILE != 0 || L.B > 512)
+    if (L.layout != QVX_LAYOUT_NATIVE || L.dtype == QVX_F32 || L.dtype == QVX_Q4 || (L.d != 64 && L.d != 128) || L.B % TILE != 0 || L.B > 512)
         return fail(dev, QVX_ERR_UNSUPPORTED,
                     "qvx_attn_decode_static: native layout, bf16 or f16, head_dim 64 or 128, block_tokens a multiple of 16 up to 512");
     const uint32_t chunk_tokens = base_chunk_tokens(CHUNK_BASE_TOKENS, L.B);

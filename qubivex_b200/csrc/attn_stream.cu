@@ -1167,7 +1167,7 @@ extern int* device_status_word(qvx_device* dev);
 // The geometries this kernel serves: native-layout pools of any dtype, blocks of whole tiles, GQA groups.
 // Everything else runs in the reference's operation order (attn_exact.cu).
 bool attn_split_supported(const Layout& L, size_t heads) {
-    if (L.layout != QVX_LAYOUT_NATIVE) return false;
+    if (L.layout != QVX_LAYOUT_NATIVE || L.dtype == QVX_Q4) return false;
     if (L.B % TILE != 0 || heads == 0 || heads % L.kvh != 0) return false;
     if (L.dtype == QVX_F32) return L.d == 64 || L.d == 128;
     return L.d == 64 || L.d == 128 || L.d == 256;

@@ -43,6 +43,7 @@ __device__ __forceinline__ bool row_target(const RowArgs& a, uint32_t r, uint32_
         block = at / a.L.B; slot = at % a.L.B;
     } else {
         uint32_t p = a.pos[r];
+        if (p == QVX_POS_NONE) return false;
         block = a.blocks[a.table_at[r] + p / a.L.B];
         slot = p % a.L.B;
     }
@@ -88,7 +89,9 @@ __global__ void __launch_bounds__(256) kv_rows_native_kernel(RowArgs a) {
         if (a.at_direct) {
             at[u] = a.at_direct[r];
         } else {
-            const uint32_t p = a.pos[r], blk = a.blocks[a.table_at[r] + p / a.L.B];
+            const uint32_t p = a.pos[r];
+            if (p == QVX_POS_NONE) continue;  // padding of the batch
+            const uint32_t blk = a.blocks[a.table_at[r] + p / a.L.B];
             // (checked before the multiplication: a wild id must not wrap into the pool)
             at[u] = blk < a.pool_blocks ? blk * a.L.B + p % a.L.B : OUT_OF_POOL;
         }
@@ -141,6 +144,8 @@ int32_t launch_kv_rows(qvx_device* dev, const Layout& L, void* pool, const float
                        const uint32_t* pos, const uint32_t* blocks, const uint32_t* table_at, size_t n,
                        size_t pool_blocks, int kind, cudaStream_t s) {
     if (n == 0) return QVX_OK;
+    if (L.dtype == QVX_Q4)
+        return launch_kv_rows_q4(dev, L, pool, k_rows, v_rows, row_stride_f32, at_direct, pos, blocks, table_at, n, pool_blocks, kind, s);
     if (n > 0x7fffffffu) return fail(dev, QVX_ERR_CORE, "kv rows: %zu rows do not fit 31 bits", n);
     RowArgs a{L, (uint8_t*)pool, k_rows, v_rows, row_stride_f32, at_direct, pos, blocks, table_at, (uint32_t)n,
               (uint32_t)std::min<size_t>(pool_blocks, 0xffffffffu), device_status_word(dev)};

@@ -12,7 +12,7 @@
 #include <deque>
 #include <unordered_set>
 
-#include "qvx_common.cuh"
+#include "q4.cuh"
 
 namespace qvx {
 
@@ -50,6 +50,9 @@ LaunchTimer::LaunchTimer(qvx_device* dev, int kind, cudaStream_t s) : dev(dev), 
         else cudaEventCreate(&e);
         return e;
     };
+    // (an event recorded in a capture cannot be waited for: launches being captured are not timed)
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) { cudaGetLastError(); return; }
     a = get(); b = get();
     cudaEventRecord(a, s);
 }
@@ -615,6 +618,17 @@ static int32_t ensure_partials(qvx_device* dev, size_t floats, size_t counters) 
 static int32_t run_attention(qvx_device* dev, qvx_tables* t, const void* pool, const float* q, float* out,
                              uint32_t variant_flags, cudaStream_t s, const float* k_new = nullptr, const float* v_new = nullptr) {
     const uint32_t variant = variant_flags & 0xffu;
+    if (t->L.dtype == QVX_Q4) {  // rows stored by their own launch, then the window kernel with nothing left out
+        if (variant == QVX_ATTN_EXACT)
+            return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no exact-order attention over a 4-bit pool");
+        if (k_new) {
+            int32_t rc = launch_kv_rows(dev, t->L, const_cast<void*>(pool), k_new, v_new, (size_t)t->L.kvh * t->L.d, nullptr, t->d_pos,
+                                        t->d_blocks, t->d_table_at, t->s, t->pool_blocks, QVX_K_APPEND, s);
+            if (rc) return rc;
+        }
+        return launch_attn_window(dev, t->L, pool, t->pool_blocks, t->heads, t->s, q, t->d_pos, t->d_blocks, t->n_blocks, t->d_table_at,
+                                  t->max_pos, 0, 0, out, s);
+    }
     bool split_ok = attn_split_supported(t->L, t->heads) && t->n_items > 0;
     if (variant == QVX_ATTN_SPLIT && !attn_split_supported(t->L, t->heads))
         return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no split attention kernel for this geometry");
@@ -647,6 +661,11 @@ size_t qvx_block_bytes(const qvx_geometry* geo) { return geometry_ok(geo) ? (siz
 
 size_t qvx_elem_offset(const qvx_geometry* geo, size_t at, int kv, size_t g, size_t i) {
     Layout L = make_layout(geo);
+    if (L.dtype == QVX_Q4) {
+        const uint32_t slot = (uint32_t)(at % L.B), e = (uint32_t)i;
+        return (at / L.B) * (size_t)L.block_bytes + g * 2 * (size_t)L.page_bytes + slot / Q4_TILE * q4_tile_bytes(L.d) +
+               q4_codes_at(L.d, slot % Q4_TILE, kv ? 1u : 0u, e >> 2) + ((e >> 1) & 1u);
+    }
     return (at / L.B) * (size_t)L.block_bytes + in_block_offset(L, (uint32_t)(at % L.B), kv ? 1u : 0u, (uint32_t)g, (uint32_t)i);
 }
 
@@ -741,7 +760,7 @@ int32_t qvx_describe(qvx_device* dev, char* out, size_t cap) {
     return QVX_OK;
 }
 
-int32_t qvx_supports(qvx_device*, uint32_t dtype) { return dtype <= QVX_F16 ? 1 : 0; }
+int32_t qvx_supports(qvx_device*, uint32_t dtype) { return dtype <= QVX_Q4 ? 1 : 0; }
 
 const char* qvx_last_error(qvx_device* dev) { return dev ? dev->last_error.c_str() : g_last_error.c_str(); }
 
@@ -950,6 +969,62 @@ int32_t qvx_block_copy(qvx_device* dev, const qvx_geometry* geo, void* pool, siz
     return launch_block_copy(dev, make_layout(geo), pool, src, dst, n, pool_blocks, (cudaStream_t)stream);
 }
 
+int32_t qvx_kv_read(qvx_device* dev, const qvx_geometry* geo, const void* pool, size_t pool_blocks, const uint32_t* from, size_t n,
+                    void* rows, uint32_t rows_dtype, void* stream) {
+    if (!dev) return QVX_ERR_SHAPE;
+    std::lock_guard<std::mutex> lk(dev->mu);
+    if (!geometry_ok(geo)) return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no KV pool of this geometry");
+    if (rows_dtype > QVX_F16) return fail(dev, QVX_ERR_ELEMENT_TYPE, "kv read: rows are f32, bf16 or f16");
+    if (n && (!pool || !from || !rows)) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in kv read: a pool, positions and rows are needed");
+    DeviceScope scope(dev->ordinal);
+    return launch_kv_read(dev, make_layout(geo), pool, pool_blocks, from, n, rows, rows_dtype, (cudaStream_t)stream);
+}
+
+int32_t qvx_attn_decode_window(qvx_device* dev, const qvx_geometry* geo, const void* pool, size_t pool_blocks, size_t heads, size_t s,
+                               const float* q, const uint32_t* pos, const uint32_t* blocks, size_t n_blocks, const uint32_t* table_at,
+                               uint32_t max_pos, uint32_t window, uint32_t sinks, float* out, void* stream) {
+    if (!dev) return QVX_ERR_SHAPE;
+    std::lock_guard<std::mutex> lk(dev->mu);
+    if (!geometry_ok(geo)) return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no KV pool of this geometry");
+    Layout L = make_layout(geo);
+    if (heads == 0 || heads % L.kvh != 0 || s > 65535)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: %zu tokens, %zu heads, %u KV heads of %u", s, heads, L.kvh, L.d);
+    const size_t groups = (heads / L.kvh + 7) / 8 * L.kvh;
+    if (!attn_window_supported(L, heads) || groups > 65535)
+        return fail(dev, QVX_ERR_UNSUPPORTED,
+                    "window attention: native layout, head_dim 64, 128 or 256, block_tokens a multiple of 16, at most 65535 groups of heads");
+    if (max_pos > 0x7fffffffu) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: max_pos %u is past 2^31 - 1", max_pos);
+    if (s == 0) return QVX_OK;
+    if (!pool || !q || !pos || !table_at || !out || (!blocks && n_blocks) || pool_blocks == 0)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: an argument is missing, or the pool holds no block");
+    if (((uintptr_t)pool | (uintptr_t)q | (uintptr_t)out) & 15u)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: pool, q and out must be 16-byte aligned");
+    DeviceScope scope(dev->ordinal);
+    return launch_attn_window(dev, L, pool, pool_blocks, heads, s, q, pos, blocks, n_blocks, table_at, max_pos, window, sinks, out,
+                              (cudaStream_t)stream);
+}
+
+int32_t qvx_head_prelude_store(qvx_device* dev, const qvx_geometry* geo, size_t heads, size_t s, const qvx_head_prelude* p, void* stream) {
+    if (!dev) return QVX_ERR_SHAPE;
+    std::lock_guard<std::mutex> lk(dev->mu);
+    if (!geometry_ok(geo)) return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no KV pool of this geometry");
+    Layout L = make_layout(geo);
+    if (heads == 0 || heads % L.kvh != 0 || (L.d & 3u) || heads + 2ull * L.kvh > 65535 * 8ull || s > 0x7fffffffu)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: %zu tokens, %zu heads, %u KV heads of %u", s, heads, L.kvh, L.d);
+    if (!p || p->dtype > QVX_F16) return fail(dev, QVX_ERR_ELEMENT_TYPE, "head prelude: projections are f32, bf16 or f16");
+    if ((p->q_norm == nullptr) != (p->k_norm == nullptr) || (p->rope && (p->rot_dim == 0 || (p->rot_dim & 1u) || p->rot_dim > L.d)))
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: both norms or neither, and an even rot_dim of at most head_dim");
+    if (s == 0) return QVX_OK;
+    if (!p->q || !p->k || !p->v || !p->pos || !p->q_out || (p->pool && (!p->table_at || (!p->blocks && p->n_blocks))))
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: an argument is missing");
+    if (p->q_stride < heads * L.d || p->k_stride < (uint64_t)L.kvh * L.d || p->v_stride < (uint64_t)L.kvh * L.d)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: a stride is shorter than a token's heads");
+    if (((uintptr_t)p->q_out | (uintptr_t)p->k_out | (uintptr_t)p->v_out | (uintptr_t)p->pool) & 15u)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: outputs and pool must be 16-byte aligned");
+    DeviceScope scope(dev->ordinal);
+    return launch_head_prelude(dev, L, heads, s, p, (cudaStream_t)stream);
+}
+
 // ---- the op with host memory ----------------------------------------------------------------------
 static bool prelude_ok(const qvx_prelude* p) {
     if (!p || !p->rope) return false;
@@ -998,8 +1073,10 @@ static int32_t paged_attention_submit(qvx_device* dev, qvx_buffer* pool, const q
     for (size_t i = 0; i < n_sync; i++)
         if (sync_to[i] / L.B >= held)
             return fail(dev, QVX_ERR_SHAPE, "shape mismatch in routed moe attention: a block past the pool's %zu", held);
-    if ((variant & 0xffu) == QVX_ATTN_SPLIT && !attn_split_supported(L, heads))
+    if ((variant & 0xffu) == QVX_ATTN_SPLIT && !attn_split_supported(L, heads) && L.dtype != QVX_Q4)
         return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no split attention kernel for this geometry");
+    if ((variant & 0xffu) == QVX_ATTN_EXACT && L.dtype == QVX_Q4)
+        return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no exact-order attention over a 4-bit pool");
     if (s == 0 && n_sync == 0) return QVX_OK;
 
     const size_t kv_out = (size_t)L.kvh * L.d, q_out = heads * L.d;

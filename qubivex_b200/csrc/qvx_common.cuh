@@ -26,7 +26,11 @@ constexpr int STATUS_POSITION_BOUND = 2;    // a position beyond the bound the c
 constexpr int STATUS_BLOCK_OUT_OF_POOL = 3; // a block id >= pool_blocks: that row or move was skipped, nothing written
 
 // ---- geometry ------------------------------------------------------------------------
-QVX_HD uint32_t elem_size(uint32_t dtype) { return dtype == QVX_F32 ? 4u : 2u; }
+// (of a 4-bit pool, whose elements share bytes: 0)
+QVX_HD uint32_t elem_size(uint32_t dtype) { return dtype == QVX_F32 ? 4u : dtype == QVX_Q4 ? 0u : 2u; }
+// A 4-bit pool's tile: 16 positions of one KV head, codes, steps and offsets of keys and values (layout: q4.cuh).
+constexpr uint32_t Q4_TILE = 16, Q4_GROUP = 32;
+QVX_HD uint32_t q4_tile_bytes(uint32_t d) { return 20u * d; }
 
 // Everything a kernel needs to address the pool, precomputed once per launch.
 struct Layout {
@@ -38,7 +42,12 @@ struct Layout {
 
 inline bool geometry_ok(const qvx_geometry* g) {
     if (!g || !g->block_tokens || !g->kv_heads || !g->head_dim) return false;
-    if (g->dtype > QVX_F16 || g->layout > QVX_LAYOUT_NATIVE) return false;
+    if (g->dtype > QVX_Q4 || g->layout > QVX_LAYOUT_NATIVE) return false;
+    if (g->dtype == QVX_Q4) {
+        if (g->layout != QVX_LAYOUT_NATIVE || g->block_tokens % Q4_TILE != 0) return false;
+        if (g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256) return false;
+        return (uint64_t)g->kv_heads * (g->block_tokens / Q4_TILE) * q4_tile_bytes(g->head_dim) < (1ull << 31);
+    }
     if (g->layout == QVX_LAYOUT_NATIVE && (g->head_dim * elem_size(g->dtype)) % 128 != 0) return false;
     // A block must stay addressable with 32-bit in-block offsets.
     uint64_t bb = 2ull * g->block_tokens * g->kv_heads * g->head_dim * elem_size(g->dtype);
@@ -52,6 +61,11 @@ inline Layout make_layout(const qvx_geometry* g) {
     L.row_bytes = L.d * L.e;
     L.page_bytes = L.B * L.row_bytes;
     L.block_bytes = 2ull * L.kvh * L.page_bytes;
+    if (L.dtype == QVX_Q4) {  // codes of one row of keys or values; half of one (block, kv head)'s tiles
+        L.row_bytes = L.d / 2;
+        L.page_bytes = L.B / Q4_TILE * (q4_tile_bytes(L.d) / 2);
+        L.block_bytes = 2ull * L.kvh * L.page_bytes;
+    }
     return L;
 }
 
@@ -195,11 +209,31 @@ struct LaunchTimer {
     ~LaunchTimer();
 };
 
+// Makes the device current for a scope and puts the caller's back.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int ordinal) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before != ordinal) cudaSetDevice(ordinal); else before = -1;
+    }
+    ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+};
+
 // Kernel entry points of the other translation units.
 int32_t launch_kv_rows(qvx_device* dev, const Layout& L, void* pool, const float* k_rows,
                        const float* v_rows, size_t row_stride_f32, const uint32_t* at_direct,
                        const uint32_t* pos, const uint32_t* blocks, const uint32_t* table_at, size_t n,
                        size_t pool_blocks, int kind, cudaStream_t s);
+int32_t launch_kv_rows_q4(qvx_device* dev, const Layout& L, void* pool, const float* k_rows, const float* v_rows,
+                          size_t row_stride_f32, const uint32_t* at_direct, const uint32_t* pos, const uint32_t* blocks,
+                          const uint32_t* table_at, size_t n, size_t pool_blocks, int kind, cudaStream_t s);
+int32_t launch_kv_read(qvx_device* dev, const Layout& L, const void* pool, size_t pool_blocks, const uint32_t* from, size_t n,
+                       void* rows, uint32_t rows_dtype, cudaStream_t s);
+int32_t launch_head_prelude(qvx_device* dev, const Layout& L, size_t heads, size_t s, const qvx_head_prelude* p, cudaStream_t stream);
+bool attn_window_supported(const Layout& L, size_t heads);
+int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, size_t pool_blocks, size_t heads, size_t s, const float* q,
+                           const uint32_t* pos, const uint32_t* blocks, size_t n_blocks, const uint32_t* table_at, uint32_t max_pos,
+                           uint32_t window, uint32_t sinks, float* out, cudaStream_t stream);
 int32_t launch_attn_prelude(qvx_device* dev, const Layout& L, size_t heads, size_t s, float* q, float* k_new, float* v_new,
                             const qvx_prelude* p, cudaStream_t stream);
 // The positions of one chunk -- the unit of the online softmax -- before long sequences double it: 576 rounded down to

@@ -23,7 +23,11 @@
 
 namespace {
 
-uint32_t elem_size(uint32_t dtype) { return dtype == QVX_F32 ? 4u : 2u; }
+// Bytes of one block.  4-bit blocks are tiles of 16 positions, 20 bytes per dimension and KV head.
+uint64_t bytes_per_block(const qvx_geometry* geo) {
+    if (geo->dtype == QVX_Q4) return 20ull * geo->head_dim * geo->kv_heads * (geo->block_tokens / 16u);
+    return 2ull * geo->block_tokens * geo->kv_heads * geo->head_dim * (geo->dtype == QVX_F32 ? 4u : 2u);
+}
 
 struct PoolCore {
     std::mutex mu;
@@ -81,7 +85,8 @@ extern "C" {
 uint64_t qvx_kvpool_blocks_for(const qvx_geometry* geo, uint64_t configured, uint64_t budget_left, uint64_t max_arena,
                                int uncapped) {
     if (!geo || !geo->block_tokens || !geo->kv_heads || !geo->head_dim) return 0;
-    uint64_t bb = 2ull * geo->block_tokens * geo->kv_heads * geo->head_dim * elem_size(geo->dtype);
+    const uint64_t bb = bytes_per_block(geo);
+    if (!bb) return 0;
     const uint64_t DEFAULT_KV_POOL = 512ull << 20, MAX_KV_POOL = 1ull << 30;  // discrete.rs:209-213
     uint64_t room = uncapped ? configured : std::min(configured ? configured : DEFAULT_KV_POOL, MAX_KV_POOL);
     room = std::min(room, std::min(budget_left, max_arena));
@@ -93,7 +98,7 @@ qvx_kvpool* qvx_kvpool_new(const qvx_geometry* geo, uint32_t blocks) {
     if (!geo || !blocks) return nullptr;
     auto core = std::make_shared<PoolCore>();
     core->geo = *geo;
-    core->block_bytes = 2ull * geo->block_tokens * geo->kv_heads * geo->head_dim * elem_size(geo->dtype);
+    core->block_bytes = bytes_per_block(geo);
     core->blocks = blocks;
     core->refs.assign(blocks, 0);
     core->free.resize(blocks);

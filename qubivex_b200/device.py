@@ -13,12 +13,13 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import Config, Geometry, KernelTimes, Prelude, TransferStats, Usage
+from ._lib import Config, Geometry, HeadPrelude, KernelTimes, Prelude, TransferStats, Usage
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, Q4 = 0, 1, 2, 3
 LAYOUT_REFERENCE, LAYOUT_NATIVE = 0, 1
 ATTN_AUTO, ATTN_SPLIT, ATTN_EXACT = 0, 1, 2
 ATTN_POOL_SETTLED = 0x100  # or-ed into a variant: see QVX_ATTN_POOL_SETTLED in include/qvx.h
+POS_NONE = 0xFFFFFFFF      # in place of a position in device memory: no token here (QVX_POS_NONE)
 KV_BLOCK = 256  # crates/qubivex-compute/src/discrete.rs:248
 
 
@@ -108,6 +109,7 @@ class CudaDevice:
         # experiments: the build whose chunk and run-length rules can be set through the environment
         self.lib = _lib.load(experiments)
         self.h = C.c_void_p()
+        self.ordinal = device
         cfg = Config(device, capacity, kv_pool, int(timing))  # timing = n: CUDA events around every n-th launch
         rc = self.lib.qvx_open(C.byref(cfg), C.byref(self.h))
         if rc:
@@ -257,6 +259,104 @@ class CudaDevice:
                                                      ptr(sync_to), n_sync, ptr(out), variant))
         return out
 
+    # -- device memory in and out: torch tensors on this device, queued on `stream` (a cudaStream_t; 0: the default stream) --
+    def _tensor(self, x, what: str, dtypes=None, numel: int | None = None, contiguous: bool = True) -> int:
+        """The address of a CUDA tensor of this device, its type, size and layout checked."""
+        if not hasattr(x, "data_ptr") or x.get_device() != self.ordinal:
+            raise ShapeError(f"{what} must be a tensor on device {self.ordinal}")
+        if contiguous and not x.is_contiguous():
+            raise ShapeError(f"{what} must be contiguous")
+        if dtypes is not None and str(x.dtype) not in dtypes:
+            raise ShapeError(f"{what} must be one of {', '.join(dtypes)}, not {x.dtype}")
+        if numel is not None and x.numel() != numel:
+            raise ShapeError(f"shape mismatch: {what} has {x.numel()} elements, {numel} are needed")
+        return x.data_ptr()
+
+    def _pool(self, pool, geo: Geometry) -> tuple[int, int]:
+        """(address, blocks) of a pool: a DeviceBuffer of this device or a contiguous tensor."""
+        bb = self.lib.qvx_block_bytes(C.byref(geo))
+        if not bb:
+            raise Unsupported("cuda backend has no KV pool of this geometry")
+        if isinstance(pool, DeviceBuffer):
+            if pool.device is not self:
+                raise DeviceError("cuda device error: the buffer belongs to another device")
+            return pool.ptr, len(pool) // bb
+        return self._tensor(pool, "pool"), pool.numel() * pool.element_size() // bb
+
+    def kv_sync(self, geo: Geometry, pool, rows, sync_to, stream: int = 0) -> None:
+        """Rows [n, 2 * kv_out] f32 (key row, value row) into the pool positions sync_to [n] (distinct)."""
+        at, blocks = self._pool(pool, geo)
+        n = sync_to.numel()
+        self.check(self.lib.qvx_kv_sync(self.h, C.byref(geo), at, blocks,
+                                        self._tensor(rows, "rows", _FLOAT32, n * 2 * geo.kv_heads * geo.head_dim),
+                                        self._tensor(sync_to, "sync_to", _INT32), n, stream))
+
+    def kv_append(self, geo: Geometry, pool, k_new, v_new, pos, blocks, table_at, stream: int = 0) -> None:
+        """Each token's new key and value row [s, kv_out] f32 at its position of its own table."""
+        at, held = self._pool(pool, geo)
+        s = pos.numel()
+        n = s * geo.kv_heads * geo.head_dim
+        self.check(self.lib.qvx_kv_append(self.h, C.byref(geo), at, held, self._tensor(k_new, "k_new", _FLOAT32, n),
+                                          self._tensor(v_new, "v_new", _FLOAT32, n), self._tensor(pos, "pos", _INT32),
+                                          self._tensor(blocks, "blocks", _INT32), self._tensor(table_at, "table_at", _INT32, s), s, stream))
+
+    def kv_read(self, geo: Geometry, pool, at, rows, stream: int = 0):
+        """rows [n, 2 * kv_out] (f32, bf16 or f16) <- what the pool positions at [n] stand for.  Returns rows."""
+        p, held = self._pool(pool, geo)
+        n = at.numel()
+        to = self._tensor(rows, "rows", _FLOATS, n * 2 * geo.kv_heads * geo.head_dim)
+        self.check(self.lib.qvx_kv_read(self.h, C.byref(geo), p, held, self._tensor(at, "at", _INT32), n, to, _FLOATS[str(rows.dtype)], stream))
+        return rows
+
+    def attn_decode_window(self, geo: Geometry, pool, heads: int, q, pos, blocks, table_at, max_pos: int, out, window: int = 0,
+                           sinks: int = 0, stream: int = 0):
+        """Decode attention over the positions j <= pos[t] with j < sinks or j > pos[t] - window (window 0: all of them),
+        on a native-layout pool of any element type.  q, out: [s, heads, head_dim] f32; pos, table_at: [s] and blocks int32
+        on the device.  Needs no tables object and keeps nothing between calls.  Returns out."""
+        at, held = self._pool(pool, geo)
+        s = pos.numel()
+        n = s * heads * geo.head_dim
+        self.check(self.lib.qvx_attn_decode_window(
+            self.h, C.byref(geo), at, held, heads, s, self._tensor(q, "q", _FLOAT32, n), self._tensor(pos, "pos", _INT32),
+            self._tensor(blocks, "blocks", _INT32), blocks.numel(), self._tensor(table_at, "table_at", _INT32, s), max_pos, window, sinks,
+            self._tensor(out, "out", _FLOAT32, n), stream))
+        return out
+
+    def head_prelude(self, geo: Geometry, heads: int, q, k, v, pos, q_out, rope=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+                     k_out=None, v_out=None, pool=None, blocks=None, table_at=None, stream: int = 0):
+        """RMS norm of every query and key head (weights [head_dim]), NeoX RoPE by row pos[t] of `rope` [rows, rot_dim]
+        ([cos.., sin..]), and the store of the key and value rows into `pool`, in one pass.  q [s, heads * head_dim], k and v
+        [s, kv_heads * head_dim]: f32, bf16 or f16, tokens may be strided (slices of one projection).  Returns q_out
+        ([s, heads, head_dim] f32); k_out and v_out likewise, where given."""
+        d = geo.head_dim
+        s, kv_out = pos.numel(), geo.kv_heads * d
+        strides = []
+        for name, x, row in (("q", q, heads * d), ("k", k, kv_out), ("v", v, kv_out)):
+            if x.dim() != 2 or x.shape[0] != s or x.shape[1] != row or (s and x.stride(1) != 1) or x.dtype != q.dtype:
+                raise ShapeError(f"shape mismatch in head prelude: {name} must be [{s}, {row}] with contiguous rows, of q's type")
+            # (a stride says nothing where there are no second rows)
+            strides.append(x.stride(0) if s > 1 else row)
+        a = HeadPrelude(self._tensor(q, "q", _FLOATS, contiguous=False), self._tensor(k, "k", contiguous=False),
+                        self._tensor(v, "v", contiguous=False), *strides, _FLOATS[str(q.dtype)], 0,
+                        None if q_norm is None else self._tensor(q_norm, "q_norm", _FLOAT32, d),
+                        None if k_norm is None else self._tensor(k_norm, "k_norm", _FLOAT32, d), eps)
+        if rope is not None:
+            if rope.dim() != 2:
+                raise ShapeError("shape mismatch in head prelude: rope must be [rows, rot_dim]")
+            a.rope, a.rope_rows, a.rot_dim = self._tensor(rope, "rope", _FLOAT32), rope.shape[0], rope.shape[1]
+        a.pos = self._tensor(pos, "pos", _INT32)
+        a.q_out = self._tensor(q_out, "q_out", _FLOAT32, s * heads * d)
+        a.k_out = None if k_out is None else self._tensor(k_out, "k_out", _FLOAT32, s * kv_out)
+        a.v_out = None if v_out is None else self._tensor(v_out, "v_out", _FLOAT32, s * kv_out)
+        if pool is not None:
+            if blocks is None or table_at is None:
+                raise ShapeError("shape mismatch in head prelude: a pool needs blocks and table_at")
+            a.pool, a.pool_blocks = self._pool(pool, geo)
+            a.blocks, a.n_blocks = self._tensor(blocks, "blocks", _INT32), blocks.numel()
+            a.table_at = self._tensor(table_at, "table_at", _INT32, s)
+        self.check(self.lib.qvx_head_prelude_store(self.h, C.byref(geo), heads, s, C.byref(a), stream))
+        return q_out
+
     def wait(self) -> None:
         rc = self.lib.qvx_wait(self.h)
         self._keep = []
@@ -268,6 +368,11 @@ class CudaDevice:
         if len(src) != len(dst):
             raise ShapeError("shape mismatch in block copy: lists differ in length")
         self.check(self.lib.qvx_block_copy_host(self.h, pool.handle, C.byref(geo), ptr(src), ptr(dst), len(src)))
+
+
+_INT32 = ("torch.int32", "torch.uint32")
+_FLOAT32 = ("torch.float32",)
+_FLOATS = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16}
 
 
 def _numel(x) -> int:
