@@ -268,8 +268,9 @@ int32_t qvx_attn_prelude(qvx_device *dev, const qvx_geometry *geo, size_t heads,
  * block_tokens a multiple of 16.  pos, blocks and table_at are device arrays of s, n_blocks and s entries, read when the
  * kernel runs: no tables object, no scratch, nothing kept between calls, so a captured launch can be replayed on changed
  * positions and tables, and launches on different streams do not disturb each other.
- * max_pos: a bound on pos[] the host knows (at most 0x7fffffff); it and the window choose how many CTAs share a token, so
- * a token's bits depend on them, never on the rest of the batch.  A token beyond max_pos gets no output row (device
+ * max_pos: a bound on pos[] the host knows (at most 0x7fffffff).  It, the window, s and heads choose how many CTAs share a
+ * token, and with that the order its sums are taken in: a token's bits do not depend on the other tokens of the call, but
+ * may on how many there are.  A token beyond max_pos gets no output row (device
  * status); one with QVX_POS_NONE gets zeros.  A table entry past n_blocks, or a block id at or past pool_blocks, is not
  * read: its positions count as not visible and the device status says so.  What lies in slots that are not visible does
  * not matter, NaN included.  Keys, values and queries that are seen are taken to be finite: an infinity among them may

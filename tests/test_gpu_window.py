@@ -174,17 +174,19 @@ def test_blocks_outside_the_pool_and_short_tables_are_reported_and_not_read(dev,
         dev.kernel_times()
 
 
-def test_a_tokens_bits_do_not_depend_on_its_batch(dev):
+def test_a_tokens_bits_do_not_depend_on_the_other_tokens(dev):
+    """Calls of one size: whatever the others are, and wherever the token stands among them."""
     for dtype in ("f32", "bf16", "q4"):
         b = Batch(dev, [900, 31, 2000, 1], 8, 2, 128, 16, dtype)
         whole = b.run(0, 0, max_pos=4000)
         again = b.run(0, 0, max_pos=4000)
         assert b.torch.equal(whole, again)
-        for t in range(4):
-            q, pos, blocks, table_at = b.args
-            one = b.torch.empty(1, 8, 128, device="cuda")
-            dev.attn_decode_window(b.geo, b.pool, 8, q[t:t + 1], pos[t:t + 1], blocks, table_at[t:t + 1], 4000, one)
-            assert b.torch.equal(one[0], whole[t])
+        q, pos, blocks, table_at = b.args
+        for order in ([3, 1, 0, 2], [0, 0, 0, 0], [2, 1, 2, 1]):
+            o = b.torch.tensor(order, device="cuda")
+            out = b.torch.empty(4, 8, 128, device="cuda")
+            dev.attn_decode_window(b.geo, b.pool, 8, q[o], pos[o], blocks, table_at[o], 4000, out)
+            assert b.torch.equal(out, whole[o])
 
 
 def test_a_captured_launch_follows_positions_and_tables(dev):
