@@ -286,8 +286,8 @@ int32_t qvx_attn_decode_window(qvx_device *dev, const qvx_geometry *geo, const v
  * value rows at pos[t] of the token's table (qvx_kv_append's place) -- one pass over the projections, which may be strided
  * slices of one fused projection, f32, bf16 or f16.  Arithmetic in f32; not the reference's summation order.
  * A token with QVX_POS_NONE is passed over; one at or past rope_rows is too, and the device status says so; a table entry
- * past n_blocks or a block id at or past pool_blocks is not stored to (device status).  Outputs and pool 16-byte
- * aligned, head_dim a multiple of 4.  q_out / k_out / v_out may be the inputs themselves where those are f32 and
+ * past n_blocks or a block id at or past pool_blocks is not stored to (device status).  Outputs, pool and
+ * rope 16-byte aligned, head_dim a multiple of 4.  q_out / k_out / v_out may be the inputs themselves where those are f32 and
  * contiguous; otherwise inputs and outputs must not overlap. */
 typedef struct qvx_head_prelude {
     const void *q, *k, *v;                 /* element (t, h, i) at t * stride + h * head_dim + i; `dtype` elements      */

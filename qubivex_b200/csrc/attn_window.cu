@@ -20,7 +20,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
-#include <type_traits>
+#include <atomic>
 
 #include "attn_ptx.cuh"
 #include "q4.cuh"
@@ -762,7 +762,7 @@ bool attn_window_supported(const Layout& L, size_t heads) {
 }
 
 template <class T, int D, int NW, int STAGES, int MIN_CTAS>
-static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, uint32_t sms, dim3 grid, cudaStream_t s) {
+static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, uint32_t sms, int ordinal, dim3 grid, cudaStream_t s) {
     auto* kernel = attn_window_kernel<T, D, NW, STAGES, MIN_CTAS>;
     using SM = WindowSmem<T, D, NW, STAGES>;
     // CTAs per cluster: as many as keep the launch within one wave of resident CTAs, and every warp in work.
@@ -774,9 +774,14 @@ static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t t
 #endif
     while (ranks < 16 && units * ranks * 2 <= slots && 2 * ranks * NW * least * T::SUB <= tiles) ranks *= 2;
     grid.x = ranks;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM::bytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> ready{0};  // devices (by ordinal) this kernel's attributes are set on
+    const uint64_t bit = ordinal < 64 ? 1ull << ordinal : 0ull;
+    if (!(ready.load(std::memory_order_acquire) & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM::bytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(NW * 32);
@@ -812,7 +817,7 @@ int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, s
     LaunchTimer timer(dev, QVX_K_ATTN, stream);
     cudaError_t e = cudaErrorInvalidValue;
 #define QVX_WINDOW(TYPE, TILE_T, DD, STG, CTAS) \
-    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, 4, STG, CTAS>(a, units, tiles, sms, grid, stream);
+    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, 4, STG, CTAS>(a, units, tiles, sms, dev->ordinal, grid, stream);
 #define QVX_COMMA ,
     QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 64>, 64, 3, 4)
     QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 128>, 128, 3, 2)

@@ -4,9 +4,7 @@
 //   y = x * (1 / sqrt(sum(x^2) / d + eps)) * w,   z_i = y_i cos_i - y_{i+r/2} sin_i,  z_{i+r/2} = y_{i+r/2} cos_i + y_i sin_i
 // for i < r/2 (r = rot_dim <= d, the rest of a head is not turned).  Values are not touched on their way to the pool.
 //
-// A warp takes a head: four consecutive elements per lane (two heads per warp at d = 64, two fours per lane at 256),
-// the sum of squares by shuffles, the partner element of a rotation read again (it is in the L1: the other half of the
-// same row).  Everything between load and store is f32; what is stored is rounded once to the pool's type.
+// Everything between load and store is f32; what is stored is rounded once to the pool's type.
 // Bound by HBM at prompt lengths and by launch latency for a few tokens.
 #include <algorithm>
 
@@ -25,7 +23,8 @@ struct HeadPreludeArgs {
     float *q_out, *k_out, *v_out;
     uint8_t* pool;
     uint64_t n_blocks;
-    uint32_t heads, s, dtype, rope_rows, rot, pool_blocks;
+    uint32_t heads, s, dtype, rope_rows, rot, pool_blocks, shift;
+    uint32_t wide;  // outputs can be written 32 bytes at a time
     float eps;
     int* status;
 };
@@ -33,136 +32,226 @@ struct HeadPreludeArgs {
 __device__ __forceinline__ float load_one(const uint8_t* p, uint32_t dtype, uint64_t i) {
     return dtype == QVX_F32 ? reinterpret_cast<const float*>(p)[i] : widen16(reinterpret_cast<const uint16_t*>(p)[i], dtype);
 }
-// Elements 4 j .. 4 j + 3 of a row.  VEC: the row starts at a multiple of four elements.
-template <bool VEC>
-__device__ __forceinline__ float4 load_four(const uint8_t* p, uint32_t dtype, uint64_t i) {
-    if constexpr (VEC) {
-        if (dtype == QVX_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-        const uint2 h = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
-        if (dtype == QVX_BF16)
-            return make_float4(__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16),
-                               __uint_as_float(h.y & 0xffff0000u));
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    } else {
-        return make_float4(load_one(p, dtype, i), load_one(p, dtype, i + 1), load_one(p, dtype, i + 2), load_one(p, dtype, i + 3));
+// Eight consecutive elements, fetched (so that the next task's are on their way while this one's are worked on) and
+// widened.  ACT: their type, read 16 bytes at a time, or ANY_ACT: the type as an argument, one by one.
+constexpr int ANY_ACT = 3;
+template <int ACT>
+struct Eight {
+    uint4 a, b;
+    __device__ __forceinline__ void fetch(const uint8_t* p, uint32_t dtype, uint64_t i) {
+        if constexpr (ACT == QVX_F32) {
+            const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + i);
+            a = __ldcs(q); b = __ldcs(q + 1);
+        } else if constexpr (ACT == ANY_ACT) {
+            a.x = __float_as_uint(load_one(p, dtype, i)); a.y = __float_as_uint(load_one(p, dtype, i + 1));
+            a.z = __float_as_uint(load_one(p, dtype, i + 2)); a.w = __float_as_uint(load_one(p, dtype, i + 3));
+            b.x = __float_as_uint(load_one(p, dtype, i + 4)); b.y = __float_as_uint(load_one(p, dtype, i + 5));
+            b.z = __float_as_uint(load_one(p, dtype, i + 6)); b.w = __float_as_uint(load_one(p, dtype, i + 7));
+        } else {
+            a = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
+        }
     }
-}
-template <bool VEC>
-__device__ __forceinline__ void store_four(float* p, uint64_t i, float4 v) {
-    if constexpr (VEC) { *reinterpret_cast<float4*>(p + i) = v; }
-    else { p[i] = v.x; p[i + 1] = v.y; p[i + 2] = v.z; p[i + 3] = v.w; }
-}
+    __device__ __forceinline__ void clear() { a = b = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void widen(float (&x)[8]) const {
+        if constexpr (ACT == QVX_F32 || ACT == ANY_ACT) {
+            x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+            x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+        } else {
+            const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if constexpr (ACT == QVX_BF16) { x[2 * k] = __uint_as_float(h[k] << 16); x[2 * k + 1] = __uint_as_float(h[k] & 0xffff0000u); }
+                else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k])); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
+            }
+        }
+    }
+};
 
 // Where token t's rows go: false when nothing is stored (no pool, or an entry that is not the pool's, which is reported).
 __device__ __forceinline__ bool pool_target(const HeadPreludeArgs& a, uint32_t t, uint32_t p, uint32_t& block, uint32_t& slot) {
     if (!a.pool) return false;
-    const uint64_t at = (uint64_t)a.table_at[t] + p / a.L.B;
+    split_position(p, a.L.B, a.shift, block, slot);
+    const uint64_t at = (uint64_t)a.table_at[t] + block;
     block = at < a.n_blocks ? a.blocks[at] : 0xffffffffu;
-    slot = p % a.L.B;
     if (block < a.pool_blocks) return true;
     atomicExch(a.status, STATUS_BLOCK_OUT_OF_POOL);
     return false;
 }
 
-// Heads of a token in order: queries, keys, values.  A warp (half a warp at D = 64) takes one.
-template <int D, bool VEC>
-__global__ void __launch_bounds__(256) head_prelude_kernel(HeadPreludeArgs a) {
-    constexpr uint32_t LPR = D == 64 ? 16 : 32, SEG = D == 256 ? 2 : 1;  // lanes per row, fours per lane
-    const uint32_t sub = threadIdx.x / LPR, l = threadIdx.x % LPR, t = blockIdx.x;
-    const uint32_t total = a.heads + 2u * a.L.kvh, h = blockIdx.y * (256u / LPR) + sub;
-    const uint32_t p = a.pos[t];
-    if (p == 0xffffffffu) return;  // padding of the batch
-    if (a.rope && p >= a.rope_rows) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) atomicExch(a.status, STATUS_POSITION_BOUND);
-        return;
-    }
-    const bool live = h < total;  // (lanes of a row past the last keep their warp company in its shuffles)
-    const uint32_t part = h < a.heads ? 0u : h < a.heads + a.L.kvh ? 1u : 2u;
-    const uint32_t g = part == 0 ? h : part == 1 ? h - a.heads : h - a.heads - a.L.kvh;
+// A task is ROWS passes of 256 / D consecutive heads of one token, all queries, all keys or all values: angles and the
+// place in the pool are worked out once, and the rows' loads are in flight together.  A lane holds eight consecutive
+// elements; rotating swaps them between lanes at a distance of half / 8 (shuffles) or, where rot_dim is not a multiple of
+// 16, reads the partners again.  The grid is what the device holds at once, and its warps go through the queries' tasks,
+// then the keys', then the values': one kind of code at a time (a warp per task spent a quarter of its time waiting for
+// instructions), weights loaded once, the next task's position on its way.  PLAIN: norms, the exchange, no pool -- queries
+// as they mostly are, with no decision left in the rows' code.
+template <int D, int ROWS, int ACT, bool PLAIN>
+__device__ __forceinline__ void prelude_tasks(const HeadPreludeArgs& a, const uint32_t part, uint32_t task, const uint32_t tasks, const uint32_t warps) {
+    constexpr uint32_t LPR = D / 8, AT_ONCE = 32 / LPR, PER_WARP = ROWS * AT_ONCE;
+    const uint32_t lane = threadIdx.x & 31u, i = lane % LPR * 8u;
+    const uint32_t heads = part == 0 ? a.heads : a.L.kvh, pieces = (heads + PER_WARP - 1) / PER_WARP;
     const uint8_t* src = part == 0 ? a.q : part == 1 ? a.k : a.v;
-    const uint64_t row = (uint64_t)t * (part == 0 ? a.q_stride : part == 1 ? a.k_stride : a.v_stride) + (uint64_t)g * D;
+    const uint64_t stride = part == 0 ? a.q_stride : part == 1 ? a.k_stride : a.v_stride;
+    float* const out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
     const float* w = part == 0 ? a.q_norm : a.k_norm;
-    const bool norm = part < 2 && w != nullptr, turn = part < 2 && a.rope != nullptr;
+    const bool norm = PLAIN || (part < 2 && w != nullptr), turn = PLAIN || (part < 2 && a.rot != 0);
     const uint32_t half = a.rot / 2;
-    float4 x[SEG], y[SEG];  // own elements, and the ones they are turned with
-    float ss = 0.f;
+    const bool exchange = PLAIN || half % 8 == 0;
+    const uint32_t h8 = half / 8, at = i / 8, from = at < h8 ? lane + h8 : at < 2 * h8 ? lane - h8 : lane;
+    if (task >= tasks) return;
+    float wv[8];
 #pragma unroll
-    for (uint32_t sg = 0; sg < SEG; sg++) {
-        x[sg] = y[sg] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const uint32_t i = 4u * (l + 32u * sg);
-        if (live) {
-            x[sg] = load_four<VEC>(src, a.dtype, row + i);
-            if (turn && i < a.rot) {
-                float* yy = &y[sg].x;
-                const uint32_t other = i < half ? i + half : i - half;
-                if (half % 4 == 0) y[sg] = load_four<VEC>(src, a.dtype, row + other);
-                else
-                    for (uint32_t k = 0; k < 4 && i + k < a.rot; k++) yy[k] = load_one(src, a.dtype, row + (i + k < half ? i + k + half : i + k - half));
-            }
+    for (int k = 0; k < 8; k++) wv[k] = norm ? __ldg(w + i + k) : 1.f;
+    Eight<ACT> ahead[ROWS];
+    auto fetch = [&](uint32_t t, uint32_t g) {
+#pragma unroll
+        for (int u = 0; u < ROWS; u++) {
+            // (lanes of a row past the last keep their warp company in its shuffles)
+            if (g + u * AT_ONCE < heads) ahead[u].fetch(src, a.dtype, (uint64_t)t * stride + (uint64_t)(g + u * AT_ONCE) * D + i);
+            else ahead[u].clear();
         }
-        ss = fmaf(x[sg].x, x[sg].x, fmaf(x[sg].y, x[sg].y, fmaf(x[sg].z, x[sg].z, fmaf(x[sg].w, x[sg].w, ss))));
-    }
+    };
+    // This lane's first head of a task; the next are AT_ONCE apart.
+    uint32_t t = task / pieces, g0 = (task - t * pieces) * PER_WARP + lane / LPR, p = a.pos[t];
+    fetch(t, g0);
+    uint32_t t_next = t, g_next = g0, p_next = p;
+    for (; task < tasks; task += warps, t = t_next, g0 = g_next, p = p_next) {
+        const uint64_t row = (uint64_t)t * stride + (uint64_t)g0 * D + i;
+        float x[ROWS][8];
 #pragma unroll
-    for (uint32_t m = LPR / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    const float r = norm ? 1.0f / sqrtf(ss * (1.0f / D) + a.eps) : 1.0f;
-    __syncwarp();  // the outputs may lie where the inputs do: every lane of the row has read what it needs
-    uint32_t block = 0, slot = 0;
-    const bool store = live && part > 0 && pool_target(a, t, p, block, slot);
-    float* out = !live ? nullptr : part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
-    const uint64_t out_row = ((uint64_t)t * (part == 0 ? a.heads : a.L.kvh) + g) * D;
-    uint8_t* dst = a.pool + (uint64_t)block * a.L.block_bytes + (uint64_t)g * 2u * a.L.page_bytes;
-#pragma unroll
-    for (uint32_t sg = 0; sg < SEG; sg++) {
-        const uint32_t i = 4u * (l + 32u * sg);
-        float v[4] = {x[sg].x, x[sg].y, x[sg].z, x[sg].w}, o[4] = {y[sg].x, y[sg].y, y[sg].z, y[sg].w};
-        if (norm) {
-            const float4 wv = make_float4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-            v[0] = v[0] * r * wv.x; v[1] = v[1] * r * wv.y; v[2] = v[2] * r * wv.z; v[3] = v[3] * r * wv.w;
+        for (int u = 0; u < ROWS; u++) ahead[u].widen(x[u]);
+        if (task + warps < tasks) {
+            t_next = (task + warps) / pieces; g_next = (task + warps - t_next * pieces) * PER_WARP + lane / LPR;
+            p_next = a.pos[t_next];
+            // (outputs may lie where the inputs do, but a task's rows are read and written by this warp alone)
+            fetch(t_next, g_next);
         }
+        if (p == QVX_POS_NONE) continue;  // padding of the batch
+        if (a.rope && p >= a.rope_rows) {
+            if (part == 0 && g0 == 0) atomicExch(a.status, STATUS_POSITION_BOUND);
+            continue;
+        }
+        float cs[8], sn[8];  // this lane's cosines and signed sines (1 and 0 past rot_dim)
+#pragma unroll
+        for (int k = 0; k < 8; k++) { cs[k] = 1.f; sn[k] = 0.f; }
         if (turn && i < a.rot) {
             const float* table = a.rope + (uint64_t)p * a.rot;
+            if (exchange) {
+                const uint32_t c = i < half ? i : i - half;
+                const float sign = i < half ? -1.f : 1.f;
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++) {
-                const uint32_t e = i + k;
-                if (e < a.rot) {
-                    const bool first = e < half;
-                    const uint32_t c = first ? e : e - half;
-                    const float other = norm ? o[k] * r * w[first ? e + half : e - half] : o[k];
-                    const float cs = table[c], sn = table[half + c];
-                    v[k] = first ? v[k] * cs - other * sn : v[k] * cs + other * sn;
+                for (int k = 0; k < 8; k += 4) {
+                    const float4 cv = __ldg(reinterpret_cast<const float4*>(table + c + k)), sv = __ldg(reinterpret_cast<const float4*>(table + half + c + k));
+                    cs[k] = cv.x; cs[k + 1] = cv.y; cs[k + 2] = cv.z; cs[k + 3] = cv.w;
+                    sn[k] = sign * sv.x; sn[k + 1] = sign * sv.y; sn[k + 2] = sign * sv.z; sn[k + 3] = sign * sv.w;
+                }
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++) {
+                    const uint32_t e = i + k;
+                    if (e < a.rot) {
+                        cs[k] = table[e < half ? e : e - half];
+                        sn[k] = e < half ? -table[half + e] : table[e];
+                    }
                 }
             }
         }
-        const float4 z = make_float4(v[0], v[1], v[2], v[3]);
-        if (out) store_four<true>(out, out_row + i, z);
-        if (a.pool == nullptr) continue;
-        if (a.L.dtype == QVX_Q4) {  // (all lanes of the warp: the groups' extremes go by shuffles)
-            __half step, offset;
-            const uint32_t codes = q4_quantise(z, step, offset);
-            if (store) {
-                const uint32_t kv = part - 1u, j = i >> 2, sl = slot % Q4_TILE;
-                uint8_t* tile = dst + (uint64_t)(slot / Q4_TILE) * q4_tile_bytes(D);
-                *reinterpret_cast<uint16_t*>(tile + q4_codes_at(D, sl, kv, j)) = (uint16_t)codes;
-                if ((j & 7u) == 0u) {
-                    *reinterpret_cast<__half*>(tile + q4_step_at(D, sl, kv, j >> 3)) = step;
-                    *reinterpret_cast<__half*>(tile + q4_offset_at(D, sl, kv, j >> 3)) = offset;
+        uint32_t block = 0, slot = 0;
+        const bool store = !PLAIN && part > 0 && pool_target(a, t, p, block, slot);
+        uint8_t* at_block = a.pool + (uint64_t)block * a.L.block_bytes;
+#pragma unroll
+        for (int u = 0; u < ROWS; u++) {
+            const uint32_t g = g0 + u * AT_ONCE;
+            const bool live = g < heads;
+            float(&v)[8] = x[u];
+            float r = 1.f;
+            if (norm) {
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) { s0 = fmaf(v[k], v[k], s0); s1 = fmaf(v[k + 1], v[k + 1], s1); }
+                float ss = s0 + s1;
+#pragma unroll
+                for (uint32_t m = LPR / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+                r = rsqrtf(fmaf(ss, 1.0f / D, a.eps));
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = v[k] * r * wv[k];
+            }
+            if (turn) {
+                float o[8];  // the elements these are turned with, normed as well
+                if (exchange) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) o[k] = __shfl_sync(0xffffffffu, v[k], from);
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k++) {
+                        const uint32_t e = i + k, other = e < half ? e + half : e - half;
+                        o[k] = 0.f;
+                        if (live && e < a.rot) {
+                            o[k] = load_one(src, a.dtype, row - i + u * AT_ONCE * D + other);
+                            if (norm) o[k] *= r * w[other];
+                        }
+                    }
+                    __syncwarp();  // (outputs may lie where the inputs do: every lane has read what it needs)
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = fmaf(v[k], cs[k], o[k] * sn[k]);
+            }
+            if ((PLAIN || out) && live) {
+                float* to = out + ((uint64_t)t * heads + g) * D + i;
+                if (a.wide) st_f32x8(to, v);
+                else {
+                    reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
                 }
             }
-        } else if (store) {
-            if (a.L.layout == QVX_LAYOUT_NATIVE) {
-                uint8_t* at = a.pool + (uint64_t)block * a.L.block_bytes + in_block_offset(a.L, slot, part - 1u, g, i);
-                if (a.L.dtype == QVX_F32) *reinterpret_cast<float4*>(at) = z;
-                else *reinterpret_cast<uint2*>(at) = make_uint2(narrow16x2(z.x, z.y, a.L.dtype), narrow16x2(z.z, z.w, a.L.dtype));
-            } else {
-                for (uint32_t k = 0; k < 4; k++) {
-                    uint8_t* at = a.pool + (uint64_t)block * a.L.block_bytes + in_block_offset(a.L, slot, part - 1u, g, i + k);
-                    if (a.L.dtype == QVX_F32) *reinterpret_cast<float*>(at) = v[k];
-                    else *reinterpret_cast<uint16_t*>(at) = narrow16(v[k], a.L.dtype);
+            if (PLAIN || part == 0 || a.pool == nullptr) continue;
+            if (a.L.dtype == QVX_Q4) {  // (all lanes of the warp: the groups' extremes go by shuffles)
+                __half step, offset;
+                const uint32_t codes = q4_quantise(v, step, offset);
+                if (store && live)
+                    Q4Place<D>(part - 1u, i).store(at_block + (uint64_t)g * 2u * a.L.page_bytes + slot / Q4_TILE * q4_tile_bytes(D), slot % Q4_TILE, codes, step, offset);
+            } else if (store && live) {
+                if (a.L.layout == QVX_LAYOUT_NATIVE) {
+                    if (a.L.dtype == QVX_F32) {
+                        *reinterpret_cast<float4*>(at_block + in_block_offset(a.L, slot, part - 1u, g, i)) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4*>(at_block + in_block_offset(a.L, slot, part - 1u, g, i + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        *reinterpret_cast<uint4*>(at_block + in_block_offset(a.L, slot, part - 1u, g, i)) =
+                            make_uint4(narrow16x2(v[0], v[1], a.L.dtype), narrow16x2(v[2], v[3], a.L.dtype), narrow16x2(v[4], v[5], a.L.dtype),
+                                       narrow16x2(v[6], v[7], a.L.dtype));
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k++) {
+                        uint8_t* to = at_block + in_block_offset(a.L, slot, part - 1u, g, i + k);
+                        if (a.L.dtype == QVX_F32) *reinterpret_cast<float*>(to) = v[k];
+                        else *reinterpret_cast<uint16_t*>(to) = narrow16(v[k], a.L.dtype);
+                    }
                 }
             }
         }
     }
+}
+
+template <int D, int ROWS, int ACT>
+__global__ void __launch_bounds__(256, 3) head_prelude_kernel(HeadPreludeArgs a) {
+    constexpr uint32_t PER_WARP = ROWS * (256 / D);
+    const uint32_t warps = gridDim.x * 8u, gw = blockIdx.x * 8u + (threadIdx.x >> 5);
+    const uint32_t q_tasks = a.s * ((a.heads + PER_WARP - 1) / PER_WARP), kv_tasks = a.s * ((a.L.kvh + PER_WARP - 1) / PER_WARP);
+    if (a.q_norm && a.rot && a.rot % 16 == 0) prelude_tasks<D, ROWS, ACT, true>(a, 0, gw, q_tasks, warps);
+    else prelude_tasks<D, ROWS, ACT, false>(a, 0, gw, q_tasks, warps);
+    // (the warps that the tasks before left out go first)
+    prelude_tasks<D, ROWS, ACT, false>(a, 1, (gw + warps - q_tasks % warps) % warps, kv_tasks, warps);
+    prelude_tasks<D, ROWS, ACT, false>(a, 2, (gw + warps - (q_tasks + kv_tasks) % warps) % warps, kv_tasks, warps);
+}
+
+template <int D, int ROWS>
+static void launch_sized(const HeadPreludeArgs& a, uint64_t warps, bool vec, uint32_t sms, cudaStream_t s) {
+    const unsigned grid = (unsigned)std::min<uint64_t>((warps + 7) / 8, 3ull * sms);
+    if (!vec) head_prelude_kernel<D, ROWS, ANY_ACT><<<grid, 256, 0, s>>>(a);
+    else if (a.dtype == QVX_F32) head_prelude_kernel<D, ROWS, QVX_F32><<<grid, 256, 0, s>>>(a);
+    else if (a.dtype == QVX_BF16) head_prelude_kernel<D, ROWS, QVX_BF16><<<grid, 256, 0, s>>>(a);
+    else head_prelude_kernel<D, ROWS, QVX_F16><<<grid, 256, 0, s>>>(a);
 }
 
 // Any other head size: one warp per head, a lane takes whole pairs, so that outputs may lie where the inputs do.
@@ -229,20 +318,25 @@ int32_t launch_head_prelude(qvx_device* dev, const Layout& L, size_t heads, size
     a.heads = (uint32_t)heads; a.s = (uint32_t)s; a.dtype = p->dtype;
     a.rope_rows = p->rope_rows; a.rot = p->rope ? p->rot_dim : 0u;
     a.pool_blocks = (uint32_t)std::min<size_t>(p->pool_blocks, 0xffffffffu);
+    a.shift = block_shift(L.B);
     a.eps = (float)p->eps;
     a.status = device_status_word(dev);
     const uint32_t e = p->dtype == QVX_F32 ? 4 : 2;
-    const bool vec = (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v) % (4 * e)) == 0 &&
-                     ((p->q_stride | p->k_stride | p->v_stride) % 4) == 0;
+    const bool vec = (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v) % 16) == 0 && ((p->q_stride | p->k_stride | p->v_stride) * e % 16) == 0;
+    a.wide = (((uintptr_t)p->q_out | (uintptr_t)p->k_out | (uintptr_t)p->v_out) % 32) == 0 ? 1u : 0u;
     const uint32_t rows = a.heads + 2u * L.kvh;
-    LaunchTimer timer(dev, QVX_K_PRELUDE, stream);
     const bool sized = L.d == 64 || L.d == 128 || L.d == 256;
-    const uint32_t per = sized && L.d == 64 ? 16 : 8;
-    const dim3 grid((unsigned)s, (rows + per - 1) / per);
-    if (!sized) head_prelude_any_kernel<<<grid, 256, 0, stream>>>(a);
-    else if (L.d == 64) { if (vec) head_prelude_kernel<64, true><<<grid, 256, 0, stream>>>(a); else head_prelude_kernel<64, false><<<grid, 256, 0, stream>>>(a); }
-    else if (L.d == 128) { if (vec) head_prelude_kernel<128, true><<<grid, 256, 0, stream>>>(a); else head_prelude_kernel<128, false><<<grid, 256, 0, stream>>>(a); }
-    else { if (vec) head_prelude_kernel<256, true><<<grid, 256, 0, stream>>>(a); else head_prelude_kernel<256, false><<<grid, 256, 0, stream>>>(a); }
+    // Fewer rows than warps the device holds: a warp each, for the least latency.
+    const uint32_t sms = (uint32_t)dev->prop.multiProcessorCount;
+    const bool few = (uint64_t)s * rows < (uint64_t)sms * 32;
+    const uint32_t per = sized ? (few ? 1u : 2u) * (256u / L.d) : 1u;
+    const uint64_t warps = (uint64_t)s * ((a.heads + per - 1) / per + 2 * ((L.kvh + per - 1) / per));
+    if (warps > 0x7fffffffull) return fail(dev, QVX_ERR_CORE, "head prelude: %zu tokens are too many for one launch", s);
+    LaunchTimer timer(dev, QVX_K_PRELUDE, stream);
+    if (!sized) head_prelude_any_kernel<<<dim3((unsigned)s, (rows + 7) / 8), 256, 0, stream>>>(a);
+    else if (L.d == 64) { if (few) launch_sized<64, 1>(a, warps, vec, sms, stream); else launch_sized<64, 2>(a, warps, vec, sms, stream); }
+    else if (L.d == 128) { if (few) launch_sized<128, 1>(a, warps, vec, sms, stream); else launch_sized<128, 2>(a, warps, vec, sms, stream); }
+    else { if (few) launch_sized<256, 1>(a, warps, vec, sms, stream); else launch_sized<256, 2>(a, warps, vec, sms, stream); }
     return check_cuda(dev, cudaGetLastError(), "head prelude launch");
 }
 

@@ -1019,8 +1019,8 @@ int32_t qvx_head_prelude_store(qvx_device* dev, const qvx_geometry* geo, size_t 
         return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: an argument is missing");
     if (p->q_stride < heads * L.d || p->k_stride < (uint64_t)L.kvh * L.d || p->v_stride < (uint64_t)L.kvh * L.d)
         return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: a stride is shorter than a token's heads");
-    if (((uintptr_t)p->q_out | (uintptr_t)p->k_out | (uintptr_t)p->v_out | (uintptr_t)p->pool) & 15u)
-        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: outputs and pool must be 16-byte aligned");
+    if (((uintptr_t)p->q_out | (uintptr_t)p->k_out | (uintptr_t)p->v_out | (uintptr_t)p->pool | (uintptr_t)p->rope) & 15u)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in head prelude: outputs, pool and rope must be 16-byte aligned");
     DeviceScope scope(dev->ordinal);
     return launch_head_prelude(dev, L, heads, s, p, (cudaStream_t)stream);
 }

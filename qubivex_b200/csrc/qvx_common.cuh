@@ -69,6 +69,17 @@ inline Layout make_layout(const qvx_geometry* g) {
     return L;
 }
 
+// Positions to blocks and slots: shifts where B is a power of two (`shift` its logarithm), divisions where not (32).
+QVX_HD uint32_t block_shift(uint32_t B) {
+    uint32_t n = 0;
+    while ((2u << n) <= B && n < 30) n++;
+    return (1u << n) == B ? n : 32u;
+}
+QVX_HD void split_position(uint32_t p, uint32_t B, uint32_t shift, uint32_t& block, uint32_t& slot) {
+    if (shift < 32u) { block = p >> shift; slot = p & (B - 1u); }
+    else { block = p / B; slot = p - block * B; }
+}
+
 // Byte offset inside one block of key (kv = 0) / value (kv = 1) element (g, i) of `slot`.
 // REFERENCE: kv_key_word / kv_value_word (crates/qubivex-compute/src/discrete.rs:317-329)
 // with KV_BLOCK generalised to B and the f32 word to one element.

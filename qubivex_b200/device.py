@@ -8,6 +8,8 @@ of libqvx_cuda.so.  Errors mirror `ComputeError` (crates/qubivex-compute/src/lib
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import types
 from dataclasses import dataclass
 
 import numpy as np
@@ -260,52 +262,56 @@ class CudaDevice:
         return out
 
     # -- device memory in and out: torch tensors on this device, queued on `stream` (a cudaStream_t; 0: the default stream) --
-    def _tensor(self, x, what: str, dtypes=None, numel: int | None = None, contiguous: bool = True) -> int:
-        """The address of a CUDA tensor of this device, its type, size and layout checked."""
-        if not hasattr(x, "data_ptr") or x.get_device() != self.ordinal:
-            raise ShapeError(f"{what} must be a tensor on device {self.ordinal}")
-        if contiguous and not x.is_contiguous():
-            raise ShapeError(f"{what} must be contiguous")
-        if dtypes is not None and str(x.dtype) not in dtypes:
-            raise ShapeError(f"{what} must be one of {', '.join(dtypes)}, not {x.dtype}")
-        if numel is not None and x.numel() != numel:
-            raise ShapeError(f"shape mismatch: {what} has {x.numel()} elements, {numel} are needed")
-        return x.data_ptr()
+    def _tensor(self, x, what: str, types, numel: int | None = None) -> int:
+        """The address of a contiguous CUDA tensor of this device, its type and size checked."""
+        if type(x) is _torch().Tensor or hasattr(x, "data_ptr"):
+            if x.get_device() == self.ordinal and x.dtype in types and x.is_contiguous() and (numel is None or x.numel() == numel):
+                return x.data_ptr()
+            raise ShapeError(f"shape mismatch: {what} must be contiguous, on device {self.ordinal}, of {' or '.join(map(str, types))}"
+                             f"{'' if numel is None else f' and {numel} elements'}; it has {x.numel()} of {x.dtype} on {x.device}")
+        raise ShapeError(f"{what} must be a tensor on device {self.ordinal}")
 
     def _pool(self, pool, geo: Geometry) -> tuple[int, int]:
         """(address, blocks) of a pool: a DeviceBuffer of this device or a contiguous tensor."""
-        bb = self.lib.qvx_block_bytes(C.byref(geo))
+        bb = self.lib.qvx_block_bytes(geo)
         if not bb:
             raise Unsupported("cuda backend has no KV pool of this geometry")
         if isinstance(pool, DeviceBuffer):
             if pool.device is not self:
                 raise DeviceError("cuda device error: the buffer belongs to another device")
             return pool.ptr, len(pool) // bb
-        return self._tensor(pool, "pool"), pool.numel() * pool.element_size() // bb
+        if pool.get_device() != self.ordinal or not pool.is_contiguous():
+            raise ShapeError(f"pool must be a contiguous tensor on device {self.ordinal}")
+        return pool.data_ptr(), pool.nbytes // bb
 
     def kv_sync(self, geo: Geometry, pool, rows, sync_to, stream: int = 0) -> None:
         """Rows [n, 2 * kv_out] f32 (key row, value row) into the pool positions sync_to [n] (distinct)."""
         at, blocks = self._pool(pool, geo)
-        n = sync_to.numel()
-        self.check(self.lib.qvx_kv_sync(self.h, C.byref(geo), at, blocks,
-                                        self._tensor(rows, "rows", _FLOAT32, n * 2 * geo.kv_heads * geo.head_dim),
-                                        self._tensor(sync_to, "sync_to", _INT32), n, stream))
+        t, n = _types(), sync_to.numel()
+        rc = self.lib.qvx_kv_sync(self.h, geo, at, blocks, self._tensor(rows, "rows", t.f32, n * 2 * geo.kv_heads * geo.head_dim),
+                                  self._tensor(sync_to, "sync_to", t.int), n, stream)
+        if rc:
+            self.check(rc)
 
     def kv_append(self, geo: Geometry, pool, k_new, v_new, pos, blocks, table_at, stream: int = 0) -> None:
         """Each token's new key and value row [s, kv_out] f32 at its position of its own table."""
         at, held = self._pool(pool, geo)
-        s = pos.numel()
+        t, s = _types(), pos.numel()
         n = s * geo.kv_heads * geo.head_dim
-        self.check(self.lib.qvx_kv_append(self.h, C.byref(geo), at, held, self._tensor(k_new, "k_new", _FLOAT32, n),
-                                          self._tensor(v_new, "v_new", _FLOAT32, n), self._tensor(pos, "pos", _INT32),
-                                          self._tensor(blocks, "blocks", _INT32), self._tensor(table_at, "table_at", _INT32, s), s, stream))
+        rc = self.lib.qvx_kv_append(self.h, geo, at, held, self._tensor(k_new, "k_new", t.f32, n), self._tensor(v_new, "v_new", t.f32, n),
+                                    self._tensor(pos, "pos", t.int), self._tensor(blocks, "blocks", t.int),
+                                    self._tensor(table_at, "table_at", t.int, s), s, stream)
+        if rc:
+            self.check(rc)
 
     def kv_read(self, geo: Geometry, pool, at, rows, stream: int = 0):
         """rows [n, 2 * kv_out] (f32, bf16 or f16) <- what the pool positions at [n] stand for.  Returns rows."""
         p, held = self._pool(pool, geo)
-        n = at.numel()
-        to = self._tensor(rows, "rows", _FLOATS, n * 2 * geo.kv_heads * geo.head_dim)
-        self.check(self.lib.qvx_kv_read(self.h, C.byref(geo), p, held, self._tensor(at, "at", _INT32), n, to, _FLOATS[str(rows.dtype)], stream))
+        t, n = _types(), at.numel()
+        to = self._tensor(rows, "rows", t.floats, n * 2 * geo.kv_heads * geo.head_dim)
+        rc = self.lib.qvx_kv_read(self.h, geo, p, held, self._tensor(at, "at", t.int), n, to, t.floats[rows.dtype], stream)
+        if rc:
+            self.check(rc)
         return rows
 
     def attn_decode_window(self, geo: Geometry, pool, heads: int, q, pos, blocks, table_at, max_pos: int, out, window: int = 0,
@@ -314,12 +320,14 @@ class CudaDevice:
         on a native-layout pool of any element type.  q, out: [s, heads, head_dim] f32; pos, table_at: [s] and blocks int32
         on the device.  Needs no tables object and keeps nothing between calls.  Returns out."""
         at, held = self._pool(pool, geo)
-        s = pos.numel()
+        t, s = _types(), pos.numel()
         n = s * heads * geo.head_dim
-        self.check(self.lib.qvx_attn_decode_window(
-            self.h, C.byref(geo), at, held, heads, s, self._tensor(q, "q", _FLOAT32, n), self._tensor(pos, "pos", _INT32),
-            self._tensor(blocks, "blocks", _INT32), blocks.numel(), self._tensor(table_at, "table_at", _INT32, s), max_pos, window, sinks,
-            self._tensor(out, "out", _FLOAT32, n), stream))
+        rc = self.lib.qvx_attn_decode_window(
+            self.h, geo, at, held, heads, s, self._tensor(q, "q", t.f32, n), self._tensor(pos, "pos", t.int),
+            self._tensor(blocks, "blocks", t.int), blocks.numel(), self._tensor(table_at, "table_at", t.int, s), max_pos, window, sinks,
+            self._tensor(out, "out", t.f32, n), stream)
+        if rc:
+            self.check(rc)
         return out
 
     def head_prelude(self, geo: Geometry, heads: int, q, k, v, pos, q_out, rope=None, q_norm=None, k_norm=None, eps: float = 1e-6,
@@ -328,33 +336,43 @@ class CudaDevice:
         ([cos.., sin..]), and the store of the key and value rows into `pool`, in one pass.  q [s, heads * head_dim], k and v
         [s, kv_heads * head_dim]: f32, bf16 or f16, tokens may be strided (slices of one projection).  Returns q_out
         ([s, heads, head_dim] f32); k_out and v_out likewise, where given."""
-        d = geo.head_dim
+        t, tensor, d = _types(), self._tensor, geo.head_dim
         s, kv_out = pos.numel(), geo.kv_heads * d
-        strides = []
-        for name, x, row in (("q", q, heads * d), ("k", k, kv_out), ("v", v, kv_out)):
-            if x.dim() != 2 or x.shape[0] != s or x.shape[1] != row or (s and x.stride(1) != 1) or x.dtype != q.dtype:
-                raise ShapeError(f"shape mismatch in head prelude: {name} must be [{s}, {row}] with contiguous rows, of q's type")
-            # (a stride says nothing where there are no second rows)
-            strides.append(x.stride(0) if s > 1 else row)
-        a = HeadPrelude(self._tensor(q, "q", _FLOATS, contiguous=False), self._tensor(k, "k", contiguous=False),
-                        self._tensor(v, "v", contiguous=False), *strides, _FLOATS[str(q.dtype)], 0,
-                        None if q_norm is None else self._tensor(q_norm, "q_norm", _FLOAT32, d),
-                        None if k_norm is None else self._tensor(k_norm, "k_norm", _FLOAT32, d), eps)
+        dtype = q.dtype
+        if dtype not in t.floats or k.dtype != dtype or v.dtype != dtype or q.shape != (s, heads * d) or k.shape != (s, kv_out) or v.shape != (s, kv_out):
+            raise ShapeError(f"shape mismatch in head prelude: q, k and v must be [{s}, {heads * d}], [{s}, {kv_out}] and [{s}, {kv_out}], of one float type")
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
+        here = self.ordinal
+        if s and (sq[1] != 1 or sk[1] != 1 or sv[1] != 1 or q.get_device() != here or k.get_device() != here or v.get_device() != here):
+            raise ShapeError(f"shape mismatch in head prelude: q, k and v need contiguous rows on device {here}")
+        a = HeadPrelude(q.data_ptr(), k.data_ptr(), v.data_ptr())
+        # (a stride says nothing where there is no second row)
+        a.q_stride, a.k_stride, a.v_stride = (sq[0], sk[0], sv[0]) if s > 1 else (heads * d, kv_out, kv_out)
+        a.dtype, a.eps = t.floats[dtype], eps
+        if q_norm is not None:
+            a.q_norm = tensor(q_norm, "q_norm", t.f32, d)
+        if k_norm is not None:
+            a.k_norm = tensor(k_norm, "k_norm", t.f32, d)
         if rope is not None:
             if rope.dim() != 2:
                 raise ShapeError("shape mismatch in head prelude: rope must be [rows, rot_dim]")
-            a.rope, a.rope_rows, a.rot_dim = self._tensor(rope, "rope", _FLOAT32), rope.shape[0], rope.shape[1]
-        a.pos = self._tensor(pos, "pos", _INT32)
-        a.q_out = self._tensor(q_out, "q_out", _FLOAT32, s * heads * d)
-        a.k_out = None if k_out is None else self._tensor(k_out, "k_out", _FLOAT32, s * kv_out)
-        a.v_out = None if v_out is None else self._tensor(v_out, "v_out", _FLOAT32, s * kv_out)
+            a.rope = tensor(rope, "rope", t.f32)
+            a.rope_rows, a.rot_dim = rope.shape
+        a.pos = tensor(pos, "pos", t.int)
+        a.q_out = tensor(q_out, "q_out", t.f32, s * heads * d)
+        if k_out is not None:
+            a.k_out = tensor(k_out, "k_out", t.f32, s * kv_out)
+        if v_out is not None:
+            a.v_out = tensor(v_out, "v_out", t.f32, s * kv_out)
         if pool is not None:
             if blocks is None or table_at is None:
                 raise ShapeError("shape mismatch in head prelude: a pool needs blocks and table_at")
             a.pool, a.pool_blocks = self._pool(pool, geo)
-            a.blocks, a.n_blocks = self._tensor(blocks, "blocks", _INT32), blocks.numel()
-            a.table_at = self._tensor(table_at, "table_at", _INT32, s)
-        self.check(self.lib.qvx_head_prelude_store(self.h, C.byref(geo), heads, s, C.byref(a), stream))
+            a.blocks, a.n_blocks = tensor(blocks, "blocks", t.int), blocks.numel()
+            a.table_at = tensor(table_at, "table_at", t.int, s)
+        rc = self.lib.qvx_head_prelude_store(self.h, geo, heads, s, a, stream)
+        if rc:
+            self.check(rc)
         return q_out
 
     def wait(self) -> None:
@@ -370,9 +388,18 @@ class CudaDevice:
         self.check(self.lib.qvx_block_copy_host(self.h, pool.handle, C.byref(geo), ptr(src), ptr(dst), len(src)))
 
 
-_INT32 = ("torch.int32", "torch.uint32")
-_FLOAT32 = ("torch.float32",)
-_FLOATS = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16}
+@functools.cache
+def _torch():
+    import torch  # by the first call that is given tensors, so it is there already
+    return torch
+
+
+@functools.cache
+def _types():
+    """The tensor types the calls on device memory take."""
+    torch = _torch()
+    return types.SimpleNamespace(f32=(torch.float32,), int=(torch.int32, torch.uint32),
+                                 floats={torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
 
 
 def _numel(x) -> int:
