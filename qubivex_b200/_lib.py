@@ -33,7 +33,7 @@ class Prelude(C.Structure):
 
 
 class HeadPrelude(C.Structure):
-    """qvx_head_prelude."""
+    """qvx_head_prelude (device.py packs it; this states its fields)."""
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
                 ("v_stride", C.c_uint64), ("dtype", C.c_uint32), ("rot_dim", C.c_uint32), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
                 ("eps", C.c_double), ("rope", C.c_void_p), ("rope_rows", C.c_uint32), ("pos", C.c_void_p), ("q_out", C.c_void_p),
@@ -104,7 +104,7 @@ PROTOTYPES = {
     "qvx_kv_read": (C.c_int32, [P, _GEO, P, C.c_size_t, P, C.c_size_t, P, C.c_uint32, P]),
     "qvx_attn_decode_window": (C.c_int32, [P, _GEO, P, C.c_size_t, C.c_size_t, C.c_size_t, P, P, P, C.c_size_t, P, C.c_uint32,
                                            C.c_uint32, C.c_uint32, P, P]),
-    "qvx_head_prelude_store": (C.c_int32, [P, _GEO, C.c_size_t, C.c_size_t, C.POINTER(HeadPrelude), P]),
+    "qvx_head_prelude_store": (C.c_int32, [P, _GEO, C.c_size_t, C.c_size_t, P, P]),
     "qvx_tables_create": (C.c_int32, [P, _GEO, C.c_size_t, C.c_size_t, C.c_size_t, P, P, C.c_size_t, P, C.POINTER(P)]),
     "qvx_tables_free": (None, [P]),
     "qvx_tables_pos": (P, [P]),

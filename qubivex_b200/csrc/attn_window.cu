@@ -716,25 +716,29 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
         for (int i = 0; i < 4; i++) own[(2 * t + (i & 1)) * D + T::dim(mt, i, lane)] = w.o[mt][i];
     if (t == 0) { ml[warp * 16 + g] = m; ml[warp * 16 + 8 + g] = l; }
     __syncthreads();
-    // The CTA's state: its warps' in order.
+    // The CTA's state: its warps' in order, weighted by 2^(m - M).  Four elements a thread at a time.
     float* cta = reinterpret_cast<float*>(smem + SM::state);
     float* out = a.out + ((uint64_t)token * a.heads + head0) * D;
-    for (uint32_t e = threadIdx.x; e < 8 * D; e += NW * 32) {
-        const uint32_t h = e / D;
-        float M = -INFINITY, L = 0.f, x = 0.f;
 #pragma unroll
-        for (int i = 0; i < NW; i++) M = fmaxf(M, ml[i * 16 + h]);
+    for (uint32_t e = threadIdx.x * 4; e < 8 * D; e += NW * 128) {
+        const uint32_t h = e / D;
+        float M = -INFINITY, L = 0.f, f[NW];
+#pragma unroll
+        for (int i = 0; i < NW; i++) { f[i] = ml[i * 16 + h]; M = fmaxf(M, f[i]); }
         const float ref = M == -INFINITY ? 0.f : M;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < NW; i++) {
-            const float f = ex2(ml[i * 16 + h] - ref);
-            L = fmaf(f, ml[i * 16 + 8 + h], L);
-            x = fmaf(f, reinterpret_cast<const float*>(smem + i * SM::ring)[e], x);
+            f[i] = ex2(f[i] - ref);
+            L = fmaf(f[i], ml[i * 16 + 8 + h], L);
+            const float4 y = *reinterpret_cast<const float4*>(smem + i * SM::ring + e * 4);
+            x.x = fmaf(f[i], y.x, x.x); x.y = fmaf(f[i], y.y, x.y); x.z = fmaf(f[i], y.z, x.z); x.w = fmaf(f[i], y.w, x.w);
         }
         if (ranks == 1) {
-            if (h < nheads && !over) out[e] = len ? x / L : 0.f;
+            if (h < nheads && !over)
+                *reinterpret_cast<float4*>(out + e) = len ? make_float4(x.x / L, x.y / L, x.z / L, x.w / L) : make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
-            cta[e] = x;
+            *reinterpret_cast<float4*>(cta + e) = x;
             if (e % D == 0) { ml[NW * 16 + h] = M; ml[NW * 16 + 8 + h] = L; }
         }
     }
@@ -744,12 +748,24 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
     for (uint32_t e = rank * (NW * 32) + threadIdx.x; e < nheads * D; e += ranks * (NW * 32)) {
         const uint32_t h = e / D, m_at = base + SM::ml + NW * 64 + 4 * h, x_at = base + SM::state + 4 * e;
         float M = -INFINITY, L = 0.f, x = 0.f;
-        for (uint32_t r = 0; r < ranks; r++) M = fmaxf(M, ld_cluster(m_at, r));
-        const float ref = M == -INFINITY ? 0.f : M;
-        for (uint32_t r = 0; r < ranks; r++) {
-            const float f = ex2(ld_cluster(m_at, r) - ref);
-            L = fmaf(f, ld_cluster(m_at + 32, r), L);
-            x = fmaf(f, ld_cluster(x_at, r), x);
+        for (uint32_t r0 = 0; r0 < ranks; r0 += 8) {  // (eight ranks' values in flight together)
+            float rm[8], rl[8], rx[8];
+#pragma unroll
+            for (uint32_t r = 0; r < 8; r++) {
+                const uint32_t from = min(r0 + r, ranks - 1);
+                rm[r] = ld_cluster(m_at, from); rl[r] = ld_cluster(m_at + 32, from); rx[r] = ld_cluster(x_at, from);
+            }
+            float most = M;
+#pragma unroll
+            for (uint32_t r = 0; r < 8; r++) most = fmaxf(most, rm[r]);
+            const float ref = most == -INFINITY ? 0.f : most, keep = ex2(M - ref);
+            L *= keep; x *= keep; M = most;
+#pragma unroll
+            for (uint32_t r = 0; r < 8; r++) {
+                const float f = r0 + r < ranks ? ex2(rm[r] - ref) : 0.f;
+                L = fmaf(f, rl[r], L);
+                x = fmaf(f, rx[r], x);
+            }
         }
         if (!over) out[e] = len ? x / L : 0.f;
     }
@@ -772,7 +788,11 @@ static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t t
     if (const char* v = getenv("QVX_WINDOW_SLOTS")) slots = (uint32_t)atol(v) * sms / 100;
     if (const char* v = getenv("QVX_WINDOW_LEAST")) least = (uint32_t)atol(v);
 #endif
-    while (ranks < 16 && units * ranks * 2 <= slots && 2 * ranks * NW * least * T::SUB <= tiles) ranks *= 2;
+    ranks = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, slots / units), 16);
+    ranks = std::min(ranks, std::max(1u, tiles / (NW * T::SUB * least)));
+#ifdef QVX_EXPERIMENTS
+    if (getenv("QVX_WINDOW_POW2")) while (ranks & (ranks - 1)) ranks--;
+#endif
     grid.x = ranks;
     static std::atomic<uint64_t> ready{0};  // devices (by ordinal) this kernel's attributes are set on
     const uint64_t bit = ordinal < 64 ? 1ull << ordinal : 0ull;

@@ -9,13 +9,14 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 import types
 from dataclasses import dataclass
 
 import numpy as np
 
 from . import _lib
-from ._lib import Config, Geometry, HeadPrelude, KernelTimes, Prelude, TransferStats, Usage
+from ._lib import Config, Geometry, KernelTimes, Prelude, TransferStats, Usage
 
 F32, BF16, F16, Q4 = 0, 1, 2, 3
 LAYOUT_REFERENCE, LAYOUT_NATIVE = 0, 1
@@ -264,12 +265,13 @@ class CudaDevice:
     # -- device memory in and out: torch tensors on this device, queued on `stream` (a cudaStream_t; 0: the default stream) --
     def _tensor(self, x, what: str, types, numel: int | None = None) -> int:
         """The address of a contiguous CUDA tensor of this device, its type and size checked."""
-        if type(x) is _torch().Tensor or hasattr(x, "data_ptr"):
+        try:
             if x.get_device() == self.ordinal and x.dtype in types and x.is_contiguous() and (numel is None or x.numel() == numel):
                 return x.data_ptr()
-            raise ShapeError(f"shape mismatch: {what} must be contiguous, on device {self.ordinal}, of {' or '.join(map(str, types))}"
-                             f"{'' if numel is None else f' and {numel} elements'}; it has {x.numel()} of {x.dtype} on {x.device}")
-        raise ShapeError(f"{what} must be a tensor on device {self.ordinal}")
+        except AttributeError:
+            raise ShapeError(f"{what} must be a tensor on device {self.ordinal}") from None
+        raise ShapeError(f"shape mismatch: {what} must be contiguous, on device {self.ordinal}, of {' or '.join(map(str, types))}"
+                         f"{'' if numel is None else f' and {numel} elements'}; it has {x.numel()} of {x.dtype} on {x.device}")
 
     def _pool(self, pool, geo: Geometry) -> tuple[int, int]:
         """(address, blocks) of a pool: a DeviceBuffer of this device or a contiguous tensor."""
@@ -345,31 +347,28 @@ class CudaDevice:
         here = self.ordinal
         if s and (sq[1] != 1 or sk[1] != 1 or sv[1] != 1 or q.get_device() != here or k.get_device() != here or v.get_device() != here):
             raise ShapeError(f"shape mismatch in head prelude: q, k and v need contiguous rows on device {here}")
-        a = HeadPrelude(q.data_ptr(), k.data_ptr(), v.data_ptr())
         # (a stride says nothing where there is no second row)
-        a.q_stride, a.k_stride, a.v_stride = (sq[0], sk[0], sv[0]) if s > 1 else (heads * d, kv_out, kv_out)
-        a.dtype, a.eps = t.floats[dtype], eps
-        if q_norm is not None:
-            a.q_norm = tensor(q_norm, "q_norm", t.f32, d)
-        if k_norm is not None:
-            a.k_norm = tensor(k_norm, "k_norm", t.f32, d)
+        if s > 1:
+            q_stride, k_stride, v_stride = sq[0], sk[0], sv[0]
+        else:
+            q_stride, k_stride, v_stride = heads * d, kv_out, kv_out
+        rope_at = rope_rows = rot_dim = at = held = n_blocks = blocks_at = tables = 0
         if rope is not None:
             if rope.dim() != 2:
                 raise ShapeError("shape mismatch in head prelude: rope must be [rows, rot_dim]")
-            a.rope = tensor(rope, "rope", t.f32)
-            a.rope_rows, a.rot_dim = rope.shape
-        a.pos = tensor(pos, "pos", t.int)
-        a.q_out = tensor(q_out, "q_out", t.f32, s * heads * d)
-        if k_out is not None:
-            a.k_out = tensor(k_out, "k_out", t.f32, s * kv_out)
-        if v_out is not None:
-            a.v_out = tensor(v_out, "v_out", t.f32, s * kv_out)
+            rope_at = tensor(rope, "rope", t.f32)
+            rope_rows, rot_dim = rope.shape
         if pool is not None:
             if blocks is None or table_at is None:
                 raise ShapeError("shape mismatch in head prelude: a pool needs blocks and table_at")
-            a.pool, a.pool_blocks = self._pool(pool, geo)
-            a.blocks, a.n_blocks = tensor(blocks, "blocks", t.int), blocks.numel()
-            a.table_at = tensor(table_at, "table_at", t.int, s)
+            at, held = self._pool(pool, geo)
+            blocks_at, n_blocks, tables = tensor(blocks, "blocks", t.int), blocks.numel(), tensor(table_at, "table_at", t.int, s)
+        a = _HEAD_PRELUDE.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride, t.floats[dtype], rot_dim,
+            0 if q_norm is None else tensor(q_norm, "q_norm", t.f32, d), 0 if k_norm is None else tensor(k_norm, "k_norm", t.f32, d), eps,
+            rope_at, rope_rows, tensor(pos, "pos", t.int), tensor(q_out, "q_out", t.f32, s * heads * d),
+            0 if k_out is None else tensor(k_out, "k_out", t.f32, s * kv_out), 0 if v_out is None else tensor(v_out, "v_out", t.f32, s * kv_out),
+            at, held, n_blocks, blocks_at, tables)
         rc = self.lib.qvx_head_prelude_store(self.h, geo, heads, s, a, stream)
         if rc:
             self.check(rc)
@@ -388,16 +387,14 @@ class CudaDevice:
         self.check(self.lib.qvx_block_copy_host(self.h, pool.handle, C.byref(geo), ptr(src), ptr(dst), len(src)))
 
 
-@functools.cache
-def _torch():
-    import torch  # by the first call that is given tensors, so it is there already
-    return torch
+# qvx_head_prelude, field by field: packing it at once costs a third of filling a ctypes structure.
+_HEAD_PRELUDE = struct.Struct("@PPPQQQIIPPdPIPPPPPNNPP")
 
 
 @functools.cache
 def _types():
     """The tensor types the calls on device memory take."""
-    torch = _torch()
+    import torch  # by the first call that is given tensors, so it is there already
     return types.SimpleNamespace(f32=(torch.float32,), int=(torch.int32, torch.uint32),
                                  floats={torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
 

@@ -71,6 +71,14 @@ def test_arguments_are_checked_before_the_library_is_called():
         dev.head_prelude(geo, 1, torch.zeros(1, 64), torch.zeros(1, 64), torch.zeros(1, 63), at, torch.zeros(1, 64))
 
 
+def test_the_packed_prelude_has_the_structures_layout():
+    from qubivex_b200 import _lib
+    n = len(_lib.HeadPrelude._fields_)
+    a = _lib.HeadPrelude.from_buffer_copy(qd._HEAD_PRELUDE.pack(*range(1, n + 1)))
+    assert C.sizeof(_lib.HeadPrelude) == qd._HEAD_PRELUDE.size
+    assert [getattr(a, name) for name, _ in _lib.HeadPrelude._fields_] == list(range(1, n + 1))
+
+
 # ---- GPU -----------------------------------------------------------------------------------------
 def _pool(torch, geo, blocks, fill=0xFF):
     return torch.full((blocks * qd.block_bytes(geo),), fill, dtype=torch.uint8, device="cuda")
