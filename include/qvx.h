@@ -272,7 +272,7 @@ int32_t qvx_attn_prelude(qvx_device *dev, const qvx_geometry *geo, size_t heads,
  * token, and with that the order its sums are taken in: a token's bits do not depend on the other tokens of the call, but
  * may on how many there are.  A token beyond max_pos gets no output row (device
  * status); one with QVX_POS_NONE gets zeros.  A table entry past n_blocks, or a block id at or past pool_blocks, is not
- * read: its positions count as not visible and the device status says so.  What lies in slots that are not visible does
+ * read: its positions count as not visible and the device status says so (a token left with none gets zeros).  What lies in slots that are not visible does
  * not matter, NaN included.  Keys, values and queries that are seen are taken to be finite: an infinity among them may
  * come out as NaN.  pool, q and out 16-byte aligned, else QVX_ERR_SHAPE.  s at most 65535. */
 int32_t qvx_attn_decode_window(qvx_device *dev, const qvx_geometry *geo, const void *pool, size_t pool_blocks,

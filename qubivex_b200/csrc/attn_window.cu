@@ -10,6 +10,10 @@
 // takes nothing but its arguments: no work list, no scratch, no counters.  It can be captured while positions and tables
 // change, and launches on several streams share nothing.
 //
+// Measured (B200, GPU time, of the measured copy bandwidth): bf16, 128 sequences, 64 query heads over 8 of 128, window 4096:
+// 308 us, 99 %; bf16, 64 sequences, 32 over 4 of 128, window 1024: 26 us, 80 %; 4 bits, 16 x 32768 positions, 32 over 4 of
+// 128: 107 us, 48 %; 4 bits, 64 x 1024-4096 positions: 54 us, 30 %.
+//
 // Data path.  Every warp has a ring of tiles of its own that its first lane fills with bulk copies, completion on
 // mbarriers; nobody waits for another warp until the states are joined.
 //
@@ -20,7 +24,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
-#include <atomic>
+#include <mutex>
 
 #include "attn_ptx.cuh"
 #include "q4.cuh"
@@ -118,15 +122,26 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // other slots is kept out of the sums.  A tile's products are summed by the tensor cores from zero and added to o in
 // f32, rounded: the tensor cores cut sums off, and a long sum kept there would drift with every tile it takes in.
 // finish: o's values in place, O^T of dimension dim(mt, i) and head 2 t + (i & 1).
+// (No asm here is volatile: a product is a function of its registers, and the compiler may place it where it likes.)
+template <int DT>
+__device__ __forceinline__ void mma_more(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (DT == QVX_BF16) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
 template <int DT>
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     const float z = 0.f;
     if constexpr (DT == QVX_BF16) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
     } else {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z));
     }
@@ -204,13 +219,13 @@ struct Tile16 {
                 mma_first<DT>(c[ks][0], q[ks], kf[0], kf[1]);
                 mma_first<DT>(c[ks][1], q[ks], kf[2], kf[3]);
             } else {
-                mma_16816<DT>(c[ks & 1][0], q[ks], kf[0], kf[1]);
-                mma_16816<DT>(c[ks & 1][1], q[ks], kf[2], kf[3]);
+                mma_more<DT>(c[ks & 1][0], q[ks], kf[0], kf[1]);
+                mma_more<DT>(c[ks & 1][1], q[ks], kf[2], kf[3]);
             }
             if constexpr (THIRD) {
                 const uint32_t a[4] = {q3[ks][0], 0u, q3[ks][1], 0u};
                 if (ks == 0) { mma_first<DT>(c3[0], a, kf[0], kf[1]); mma_first<DT>(c3[1], a, kf[2], kf[3]); }
-                else { mma_16816<DT>(c3[0], a, kf[0], kf[1]); mma_16816<DT>(c3[1], a, kf[2], kf[3]); }
+                else { mma_more<DT>(c3[0], a, kf[0], kf[1]); mma_more<DT>(c3[1], a, kf[2], kf[3]); }
             }
         }
 #pragma unroll
@@ -235,9 +250,9 @@ struct Tile16 {
             ldmatrix_x4_trans(stage + BYTES / 2 + row * (D * 2) + (((2 * mt + chunk) ^ (row & 7u)) << 4), vf);
             vf[0] &= m0; vf[1] &= m0; vf[2] &= m1; vf[3] &= m1;
             float x[4];
-            if constexpr (THIRD) { mma_first<DT>(x, vf, t0, t1); mma_16816<DT>(x, vf, l0, l1); }
+            if constexpr (THIRD) { mma_first<DT>(x, vf, t0, t1); mma_more<DT>(x, vf, l0, l1); }
             else mma_first<DT>(x, vf, l0, l1);
-            mma_16816<DT>(x, vf, h0, h1);
+            mma_more<DT>(x, vf, h0, h1);
             rescale_add(o[mt], x, a0, a1);
         }
     }
@@ -247,7 +262,7 @@ struct Tile16 {
 
 // f32 pools: both operands as a tf32 value and its tf32 remainder (22 bits together).  Tiles of 8 positions.
 __device__ __forceinline__ void mma_1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -342,9 +357,12 @@ struct Tile32 {
 // them, is made of (1.9e-4 of the result at 20 000 positions); codes less 8 and offsets plus 8 steps have no such
 // growth.  Bits 0..3 or 4..7 under f16's 1024 are 1024 + c or 1024 + 16 c, and one subtraction, or one multiply-add, makes
 // them c - 8.
-// A stage is two tiles: what is done once per stage (maxima, their exponent, the queue's upkeep) is a third of a tile's
-// instructions, and two tiles' chains of dependent products run beside each other.  The queries' fragments stay in shared
-// memory: 32 registers less let 16 warps live on an SM instead of 12.
+// A stage is two tiles: what is done once per stage (maxima, the ring's upkeep) is shared, and two tiles' chains of
+// dependent products run beside each other.  The queries' fragments stay in shared memory, 32 registers less.
+// Bound by instructions, not by memory: about 480 a tile of 2560 bytes (d = 128), of which the masks and byte
+// permutations and the half-precision arithmetic go at half rate and a 16 x 8 x 16 product takes 8 cycles beside which
+// little else issues; 250 cycles a tile and SM where HBM asks for 111.  12 warps an SM without spills do more than 16 with
+// 76 bytes of them (107 us against 117 for 16 x 32768 positions, 32 over 4 heads), and two stages a warp as much as three.
 template <int D>
 struct TileQ4 {
     static constexpr uint32_t TP = 16, SUB = 2, PER = 4, BYTES = 20 * D, Q_SMEM = D * 32;
@@ -415,7 +433,7 @@ struct TileQ4 {
             lds_words<NG>(tile + (g + 8 * h) * (D / 2) + t * (4 * NG), w[n]);
             lds_words<NG>(tile + 16 * D + (t + 4 * h) * (4 * NG), st[n]);
             const uint32_t zk = 2 * t < NG ? lds32(tile + 18 * D + (g + 8 * h) * (2 * NG) + 4 * t) : 0u;
-            asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+            asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
                          : "=f"(zc[n][0]), "=f"(zc[n][1]), "=f"(zc[n][2]), "=f"(zc[n][3]) : "r"(qs[0]), "r"(qs[1]), "r"(zk), "f"(0.f));
         }
 #pragma unroll
@@ -428,7 +446,7 @@ struct TileQ4 {
                 float c[4];
                 const uint32_t x = w[n][G], y = x >> 8;
                 mma_first<QVX_F16>(c, q0, x & 0x000f000fu, x & 0x00f000f0u);
-                mma_16816<QVX_F16>(c, q1, y & 0x000f000fu, y & 0x00f000f0u);
+                mma_more<QVX_F16>(c, q1, y & 0x000f000fu, y & 0x00f000f0u);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&st[n][G]));
                 const P2 step = pair_of(f.x, f.y);
                 total[n] = fma2(step, pair_of(c[0], c[1]), total[n]);
@@ -445,7 +463,7 @@ struct TileQ4 {
     __device__ __forceinline__ void values(uint32_t stage, uint32_t lane, const float (&p)[8], uint32_t seen, float a0, float a1) {
         const uint32_t g = lane >> 2, t = lane & 3u;
         uint32_t st[4][NG], s2[4], z2[4];
-        __half2 top = __float2half2_rn(0.f);
+        uint32_t any = 0;
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const uint32_t tile = stage + (n >> 1) * BYTES, pair = (t + 4 * (n & 1)) * (4 * NG);
@@ -459,21 +477,30 @@ struct TileQ4 {
                 for (int G = 0; G < NG; G++) st[n][G] &= m;
             }
 #pragma unroll
-            for (int G = 0; G < NG; G++) top = __hmax2(top, *reinterpret_cast<const __half2*>(&st[n][G]));
+            for (int G = 0; G < NG; G++) any |= st[n][G];
         }
         // P s in f16, the weights times 2^14: up to 2^15 while the steps are below 2, and 22 bits of the greatest of them are
-        // kept down to steps of f16's least normal numbers.  Greater steps are brought below 2 by a power of two of their own.
-        const uint32_t bits = max((uint32_t)__half_as_ushort(__low2half(top)), (uint32_t)__half_as_ushort(__high2half(top)));
-        const uint32_t e = min(__reduce_max_sync(0xffffffffu, bits) >> 10, 30u);
+        // kept down to steps of f16's least normal numbers.  Greater steps (bit 14, the exponent's highest, set) are brought
+        // below 2 by a power of two of their own, that of the greatest seen so far.
         float b0 = a0, b1 = a1;
-        if (e > se) {
-            const float f = pow2i((int)se - (int)e);
-            b0 *= f; b1 *= f;
-            se = e;
+        const bool large = __any_sync(0xffffffffu, (any & 0x40004000u) != 0) || se > 15;
+        if (large) {
+            __half2 top = __float2half2_rn(0.f);
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int G = 0; G < NG; G++) { const uint32_t v = st[n][G] & 0x7fff7fffu; top = __hmax2(top, *reinterpret_cast<const __half2*>(&v)); }
+            const uint32_t bits = max((uint32_t)__half_as_ushort(__low2half(top)), (uint32_t)__half_as_ushort(__high2half(top)));
+            const uint32_t e = min(__reduce_max_sync(0xffffffffu, bits) >> 10, 30u);
+            if (e > se) {
+                const float f = pow2i((int)se - (int)e);
+                b0 *= f; b1 *= f;
+                se = e;
+            }
         }
         // z + 8 s = zh + zl.
         uint32_t zh[4], zl[4];
-        if (se > 15) {
+        if (large) {
             const __half2 unit = __half2half2(__float2half_rn(pow2i(15 - (int)se)));
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -502,9 +529,9 @@ struct TileQ4 {
             const uint32_t za[4] = {zh[0], zl[0], zh[1], zl[1]}, zb[4] = {zh[2], zl[2], zh[3], zl[3]};
             float x[4];
             mma_first<QVX_F16>(x, za, pl[0], pl[1]);
-            mma_16816<QVX_F16>(x, zb, pl[2], pl[3]);
-            mma_16816<QVX_F16>(x, za, ph[0], ph[1]);
-            mma_16816<QVX_F16>(x, zb, ph[2], ph[3]);
+            mma_more<QVX_F16>(x, zb, pl[2], pl[3]);
+            mma_more<QVX_F16>(x, za, ph[0], ph[1]);
+            mma_more<QVX_F16>(x, zb, ph[2], ph[3]);
             rescale_add(z, x, a0, a1);
         }
         // Codes: rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each tile, the lane's unit of each; a row's words hold two groups each.
@@ -538,9 +565,9 @@ struct TileQ4 {
                 const uint32_t v0[4] = {low_code(x), high_code(x), low_code(y), high_code(y)};
                 const uint32_t v1[4] = {low_code(x8), high_code(x8), low_code(y8), high_code(y8)};
                 if (i == 0) { mma_first<QVX_F16>(x0, v0, bl[0], bl[1]); mma_first<QVX_F16>(x1, v1, bl[0], bl[1]); }
-                else { mma_16816<QVX_F16>(x0, v0, bl[2], bl[3]); mma_16816<QVX_F16>(x1, v1, bl[2], bl[3]); }
-                mma_16816<QVX_F16>(x0, v0, bh[2 * i], bh[2 * i + 1]);
-                mma_16816<QVX_F16>(x1, v1, bh[2 * i], bh[2 * i + 1]);
+                else { mma_more<QVX_F16>(x0, v0, bl[2], bl[3]); mma_more<QVX_F16>(x1, v1, bl[2], bl[3]); }
+                mma_more<QVX_F16>(x0, v0, bh[2 * i], bh[2 * i + 1]);
+                mma_more<QVX_F16>(x1, v1, bh[2 * i], bh[2 * i + 1]);
             }
             rescale_add(o[2 * G], x0, b0, b1);
             rescale_add(o[2 * G + 1], x1, b0, b1);
@@ -620,6 +647,10 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
     }
     __syncwarp();
     const uint64_t policy = l2_policy_evict_first();
+    // Of the warp's tiles, plain_from .. plain_upto - 1 are visible to the last position: those between the tile the window
+    // begins in and the tile the sequence ends in (the sinks' are few and looked at).
+    const uint32_t wide_from = ns + (win > w0 * T::TP ? 1u : 0u), wide_upto = tiles - (len % T::TP != 0 && tiles > 0 ? 1u : 0u);
+    const uint32_t plain_from = wide_from > me ? (wide_from - me + step - 1) / step : 0u, plain_upto = wide_upto > me ? (wide_upto - me + step - 1) / step : 0u;
     auto tile_of = [&](uint32_t i) { const uint32_t j = me + i * step; return j < ns ? j : w0 + (j - ns); };
     // Lane i mod 32 looks up where the warp's i-th tile lies and issues its copy; the next 32 tiles' block ids are on their
     // way while these are in use.  An id that is not the pool's is noted in `foreign`: the copy then brings the pool's first
@@ -668,18 +699,17 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
         float s[N];
         w.scores(at, base + SM::q, lane, s);
         uint32_t seen = (1u << N) - 1u;
-#pragma unroll
-        for (int u = 0; u < (int)T::SUB; u++) {
-            const uint32_t i = done * T::SUB + u, first = tile_of(i) * T::TP;
+        if (done * T::SUB < plain_from || (done + 1) * T::SUB > plain_upto || (foreign | foreign_before) != 0) {
             // (issuing runs at most one batch of 32 ids ahead of this)
-            const uint32_t upto = min((done + STAGES) * T::SUB - 1u, (rounds - 1u) * T::SUB);
-            const bool alien = ((i >> 5) == (upto >> 5) ? foreign : foreign_before) >> (i & 31u) & 1u;
-            const bool none = i >= mine || alien;
-            if (none || first + T::TP > len || !(first >= win || first + T::TP <= sink_end)) {
+            const uint32_t issued = min((done + STAGES) * T::SUB - 1u, (rounds - 1u) * T::SUB);
+#pragma unroll
+            for (int u = 0; u < (int)T::SUB; u++) {
+                const uint32_t i = done * T::SUB + u, first = tile_of(i) * T::TP;
+                const bool alien = ((i >> 5) == (issued >> 5) ? foreign : foreign_before) >> (i & 31u) & 1u;
 #pragma unroll
                 for (int k = 0; k < (int)PER; k++) {
                     const uint32_t j = first + 2 * t + (k & 1) + 8 * (k >> 1);
-                    if (none || !(j < len && (j < sink_end || j >= win))) { s[u * PER + k] = -INFINITY; seen &= ~(1u << (u * PER + k)); }
+                    if (i >= mine || alien || !(j < len && (j < sink_end || j >= win))) { s[u * PER + k] = -INFINITY; seen &= ~(1u << (u * PER + k)); }
                 }
             }
         }
@@ -736,7 +766,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
         }
         if (ranks == 1) {
             if (h < nheads && !over)
-                *reinterpret_cast<float4*>(out + e) = len ? make_float4(x.x / L, x.y / L, x.z / L, x.w / L) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(out + e) = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
         } else {
             *reinterpret_cast<float4*>(cta + e) = x;
             if (e % D == 0) { ml[NW * 16 + h] = M; ml[NW * 16 + 8 + h] = L; }
@@ -767,7 +797,7 @@ __global__ void __launch_bounds__(NW * 32, MIN_CTAS) attn_window_kernel(WindowAr
                 x = fmaf(f, rx[r], x);
             }
         }
-        if (!over) out[e] = len ? x / L : 0.f;
+        if (!over) out[e] = L == 0.f ? 0.f : x / L;
     }
     cluster_sync_all();  // nobody leaves while its shared memory is being read
 }
@@ -777,40 +807,55 @@ bool attn_window_supported(const Layout& L, size_t heads) {
     return L.d == 64 || L.d == 128 || L.d == 256;
 }
 
+// What one of the kernels is on one device: its attributes set, and how many clusters of each size the device holds at once
+// (not its slots over the size: a cluster lies within one of the chip's groups of SMs).
+struct WindowKernel {
+    std::mutex mu;
+    bool ready = false;
+    uint32_t held[17] = {};
+};
+
 template <class T, int D, int NW, int STAGES, int MIN_CTAS>
-static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, uint32_t sms, int ordinal, dim3 grid, cudaStream_t s) {
+static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, int ordinal, dim3 grid, cudaStream_t s) {
     auto* kernel = attn_window_kernel<T, D, NW, STAGES, MIN_CTAS>;
     using SM = WindowSmem<T, D, NW, STAGES>;
-    // CTAs per cluster: as many as keep the launch within one wave of resident CTAs, and every warp in work.
-    uint32_t ranks = 1;
-    uint32_t slots = MIN_CTAS * sms, least = 1;
-#ifdef QVX_EXPERIMENTS
-    if (const char* v = getenv("QVX_WINDOW_SLOTS")) slots = (uint32_t)atol(v) * sms / 100;
-    if (const char* v = getenv("QVX_WINDOW_LEAST")) least = (uint32_t)atol(v);
-#endif
-    ranks = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, slots / units), 16);
-    ranks = std::min(ranks, std::max(1u, tiles / (NW * T::SUB * least)));
-#ifdef QVX_EXPERIMENTS
-    if (getenv("QVX_WINDOW_POW2")) while (ranks & (ranks - 1)) ranks--;
-#endif
-    grid.x = ranks;
-    static std::atomic<uint64_t> ready{0};  // devices (by ordinal) this kernel's attributes are set on
-    const uint64_t bit = ordinal < 64 ? 1ull << ordinal : 0ull;
-    if (!(ready.load(std::memory_order_acquire) & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM::bytes);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        ready.fetch_or(bit, std::memory_order_release);
-    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
     cfg.blockDim = dim3(NW * 32);
     cfg.dynamicSmemBytes = SM::bytes;
-    cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
+    static WindowKernel on[64];
+    if (ordinal < 0 || ordinal >= 64) return cudaErrorInvalidDevice;
+    WindowKernel& k = on[ordinal];
+    {
+        std::lock_guard<std::mutex> lk(k.mu);
+        if (!k.ready) {
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM::bytes);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            for (uint32_t r = 1; e == cudaSuccess && r <= 16; r = r < 8 ? r + 1 : r + 8) {
+                int n = 0;
+                cfg.gridDim = dim3(r, 1024); at[0].val.clusterDim.x = r;
+                e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+                k.held[r] = n > 0 ? (uint32_t)n : 0u;
+            }
+            if (e != cudaSuccess) return e;
+            k.ready = true;
+        }
+    }
+    // CTAs per cluster: as many as leave every cluster resident at once and every warp in work.  (64 long 4-bit sequences:
+    // 107 us with clusters of 6, 115 with 4, 134 with 8, which come in two waves.)
+    uint32_t ranks = 1;
+    for (uint32_t r = 2; r <= 16; r = r < 8 ? r + 1 : r + 8)
+        if (units <= k.held[r] && r * NW * T::SUB <= tiles) ranks = r;
+#ifdef QVX_EXPERIMENTS
+    if (const char* v = getenv("QVX_WINDOW_RANKS")) ranks = (uint32_t)atol(v);
+#endif
+    grid.x = ranks;
+    cfg.gridDim = grid;
+    cfg.stream = s;
+    at[0].val.clusterDim.x = ranks;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
@@ -831,13 +876,13 @@ int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, s
     a.status = device_status_word(dev);
     uint64_t most = (uint64_t)max_pos + 1;  // positions a token of this call may see
     if (window) most = std::min(most, (uint64_t)window + sinks);
-    const uint32_t tiles = (uint32_t)((most + tp - 1) / tp), sms = (uint32_t)dev->prop.multiProcessorCount;
+    const uint32_t tiles = (uint32_t)((most + tp - 1) / tp);
     const dim3 grid(1, L.kvh * a.groups_per_kv, (unsigned)s);
     const uint64_t units = (uint64_t)grid.y * grid.z;
     LaunchTimer timer(dev, QVX_K_ATTN, stream);
     cudaError_t e = cudaErrorInvalidValue;
 #define QVX_WINDOW(TYPE, TILE_T, DD, STG, CTAS) \
-    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, 4, STG, CTAS>(a, units, tiles, sms, dev->ordinal, grid, stream);
+    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, 4, STG, CTAS>(a, units, tiles, dev->ordinal, grid, stream);
 #define QVX_COMMA ,
     QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 64>, 64, 3, 4)
     QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 128>, 128, 3, 2)
@@ -848,8 +893,8 @@ int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, s
     QVX_WINDOW(QVX_F32, Tile32<64>, 64, 3, 4)
     QVX_WINDOW(QVX_F32, Tile32<128>, 128, 3, 2)
     QVX_WINDOW(QVX_F32, Tile32<256>, 256, 3, 1)
-    QVX_WINDOW(QVX_Q4, TileQ4<64>, 64, 2, 6)
-    QVX_WINDOW(QVX_Q4, TileQ4<128>, 128, 2, 4)
+    QVX_WINDOW(QVX_Q4, TileQ4<64>, 64, 2, 4)
+    QVX_WINDOW(QVX_Q4, TileQ4<128>, 128, 2, 3)
     QVX_WINDOW(QVX_Q4, TileQ4<256>, 256, 2, 2)
 #undef QVX_COMMA
 #undef QVX_WINDOW
