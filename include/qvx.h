@@ -53,7 +53,8 @@ extern "C" {
  * z + s c: 5 bits an element (the numerics of GGUF's Q4_1).  z is the group's least value rounded down, s is
  * (greatest - z) / 15 rounded up, so a stored element is off by at most s / 2; a group with a NaN, an infinity or a value
  * beyond 65504 stands for NaN.  Pools only, native layout only: block_tokens a multiple of 16, head_dim 64, 128 or 256;
- * rows go in and come out as f32 (or 16-bit, qvx_kv_read). */
+ * the pool 16-byte aligned; rows go in as f32 and come out as f32 or 16-bit (qvx_kv_read).  Every call that takes a
+ * geometry takes this one, but qvx_attn_decode_static and the exact-order variant (QVX_ERR_UNSUPPORTED). */
 #define QVX_Q4 3
 
 /* The reference's block: keys [kv_head][d][B] then values [B][kv_head][d]
@@ -172,7 +173,7 @@ int32_t qvx_kv_append(qvx_device *dev, const qvx_geometry *geo, void *pool, size
  * nearest: key row, value row) becomes what pool position from[r] = block * block_tokens + slot stands for.  The reverse
  * of qvx_kv_sync, for any pool: what a host cache, another pool or a prompt's attention takes back from a 4-bit or 16-bit
  * cache.  No counterpart in the reference, whose host cache holds every row.  A row whose block is at or past
- * pool_blocks is left as it was (device status, as above). */
+ * pool_blocks is left as it was (device status, as above).  The pool 16-byte aligned. */
 int32_t qvx_kv_read(qvx_device *dev, const qvx_geometry *geo, const void *pool, size_t pool_blocks,
                     const uint32_t *from, size_t n, void *rows, uint32_t rows_dtype, void *stream);
 
@@ -270,10 +271,10 @@ int32_t qvx_attn_prelude(qvx_device *dev, const qvx_geometry *geo, size_t heads,
  * positions and tables, and launches on different streams do not disturb each other.
  * max_pos: a bound on pos[] the host knows (at most 0x7fffffff).  It, the window, s and heads choose how many CTAs share a
  * token, and with that the order its sums are taken in: a token's bits do not depend on the other tokens of the call, but
- * may on how many there are.  A token beyond max_pos gets no output row (device
- * status); one with QVX_POS_NONE gets zeros.  A table entry past n_blocks, or a block id at or past pool_blocks, is not
- * read: its positions count as not visible and the device status says so (a token left with none gets zeros).  What lies in slots that are not visible does
- * not matter, NaN included.  Keys, values and queries that are seen are taken to be finite: an infinity among them may
+ * may on how many there are.  A token beyond max_pos gets no output row (device status); one with QVX_POS_NONE gets
+ * zeros.  A table entry past n_blocks, or a block id at or past pool_blocks, is not read: its positions count as not
+ * visible and the device status says so (a token left with none gets zeros).  What lies in slots that are not visible
+ * does not matter, NaN included.  Keys, values and queries that are seen are taken to be finite: an infinity among them may
  * come out as NaN.  pool, q and out 16-byte aligned, else QVX_ERR_SHAPE.  s at most 65535. */
 int32_t qvx_attn_decode_window(qvx_device *dev, const qvx_geometry *geo, const void *pool, size_t pool_blocks,
                                size_t heads, size_t s, const float *q, const uint32_t *pos, const uint32_t *blocks,
@@ -288,7 +289,7 @@ int32_t qvx_attn_decode_window(qvx_device *dev, const qvx_geometry *geo, const v
  * A token with QVX_POS_NONE is passed over; one at or past rope_rows is too, and the device status says so; a table entry
  * past n_blocks or a block id at or past pool_blocks is not stored to (device status).  Outputs, pool and
  * rope 16-byte aligned, head_dim a multiple of 4.  q_out / k_out / v_out may be the inputs themselves where those are f32 and
- * contiguous; otherwise inputs and outputs must not overlap. */
+ * contiguous; otherwise inputs and outputs must not overlap.  No two tokens of a call may have the same place in the pool. */
 typedef struct qvx_head_prelude {
     const void *q, *k, *v;                 /* element (t, h, i) at t * stride + h * head_dim + i; `dtype` elements      */
     uint64_t q_stride, k_stride, v_stride; /* elements from one token to the next                                   */

@@ -862,7 +862,10 @@ static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t t
 int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, size_t pool_blocks, size_t heads, size_t s, const float* q,
                            const uint32_t* pos, const uint32_t* blocks, size_t n_blocks, const uint32_t* table_at, uint32_t max_pos,
                            uint32_t window, uint32_t sinks, float* out, cudaStream_t stream) {
+    if (max_pos > 0x7fffffffu) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: max_pos %u is past 2^31 - 1", max_pos);
     if (s == 0) return QVX_OK;
+    if (((uintptr_t)pool | (uintptr_t)q | (uintptr_t)out) & 15u)
+        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: pool, q and out must be 16-byte aligned");
     const uint32_t tp = L.dtype == QVX_F32 ? 8 : 16;
     WindowArgs a{};
     a.pool = (const uint8_t*)pool; a.q = q; a.out = out; a.pos = pos; a.blocks = blocks; a.table_at = table_at;

@@ -94,6 +94,7 @@ int32_t launch_kv_rows_q4(qvx_device* dev, const Layout& L, void* pool, const fl
                           size_t row_stride_f32, const uint32_t* at_direct, const uint32_t* pos, const uint32_t* blocks,
                           const uint32_t* table_at, size_t n, size_t pool_blocks, int kind, cudaStream_t s) {
     if (n > 0x7fffffffu) return fail(dev, QVX_ERR_CORE, "kv rows: %zu rows do not fit 31 bits", n);
+    if ((uintptr_t)pool & 15u) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in kv rows: a 4-bit pool must be 16-byte aligned");
     const uint32_t n_row = (L.kvh * (L.d / 8) * 2u + 31u) / 32u;
     // Lines of warps, one per piece of a row: as many as there are rows for, or as the device holds (24 warps an SM).
     const uint64_t held = std::max<uint64_t>(1, 24ull * dev->prop.multiProcessorCount / n_row);

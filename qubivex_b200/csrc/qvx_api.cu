@@ -976,6 +976,7 @@ int32_t qvx_kv_read(qvx_device* dev, const qvx_geometry* geo, const void* pool, 
     if (!geometry_ok(geo)) return fail(dev, QVX_ERR_UNSUPPORTED, "cuda backend has no KV pool of this geometry");
     if (rows_dtype > QVX_F16) return fail(dev, QVX_ERR_ELEMENT_TYPE, "kv read: rows are f32, bf16 or f16");
     if (n && (!pool || !from || !rows)) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in kv read: a pool, positions and rows are needed");
+    if ((uintptr_t)pool & 15u) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in kv read: the pool must be 16-byte aligned");
     DeviceScope scope(dev->ordinal);
     return launch_kv_read(dev, make_layout(geo), pool, pool_blocks, from, n, rows, rows_dtype, (cudaStream_t)stream);
 }
@@ -993,12 +994,9 @@ int32_t qvx_attn_decode_window(qvx_device* dev, const qvx_geometry* geo, const v
     if (!attn_window_supported(L, heads) || groups > 65535)
         return fail(dev, QVX_ERR_UNSUPPORTED,
                     "window attention: native layout, head_dim 64, 128 or 256, block_tokens a multiple of 16, at most 65535 groups of heads");
-    if (max_pos > 0x7fffffffu) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: max_pos %u is past 2^31 - 1", max_pos);
     if (s == 0) return QVX_OK;
     if (!pool || !q || !pos || !table_at || !out || (!blocks && n_blocks) || pool_blocks == 0)
         return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: an argument is missing, or the pool holds no block");
-    if (((uintptr_t)pool | (uintptr_t)q | (uintptr_t)out) & 15u)
-        return fail(dev, QVX_ERR_SHAPE, "shape mismatch in window attention: pool, q and out must be 16-byte aligned");
     DeviceScope scope(dev->ordinal);
     return launch_attn_window(dev, L, pool, pool_blocks, heads, s, q, pos, blocks, n_blocks, table_at, max_pos, window, sinks, out,
                               (cudaStream_t)stream);

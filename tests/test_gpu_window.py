@@ -305,3 +305,54 @@ def test_a_4_bit_pool_through_the_ordinary_calls(dev, d):
         assert np.array_equal(again, out)
     finally:
         buf.free()
+
+
+def test_a_misaligned_query_of_the_ordinary_call_is_refused(dev):
+    import ctypes as C
+
+    import torch
+    geo = qd.geometry(16, 2, 64, qd.Q4)
+    pool = torch.zeros(4 * qd.block_bytes(geo), dtype=torch.uint8, device="cuda")
+    pos, blocks, at = np.array([5], np.uint32), np.array([1], np.uint32), np.zeros(1, np.uint32)
+    tables = C.c_void_p()
+    dev.check(dev.lib.qvx_tables_create(dev.h, geo, 4, 8, 1, qd.ptr(pos), qd.ptr(blocks), 1, qd.ptr(at), C.byref(tables)))
+    x, out = torch.zeros(520, device="cuda"), torch.zeros(512, device="cuda")
+    with pytest.raises(qd.ShapeError):
+        dev.check(dev.lib.qvx_attn_decode(dev.h, tables, pool.data_ptr(), x.data_ptr() + 4, out.data_ptr(), qd.ATTN_AUTO, None))
+    dev.check(dev.lib.qvx_attn_decode(dev.h, tables, pool.data_ptr(), x.data_ptr(), out.data_ptr(), qd.ATTN_AUTO, None))
+    torch.cuda.synchronize()
+    dev.lib.qvx_tables_free(tables)
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from qubivex_b200 import device as qd
+dev = qd.CudaDevice(0, timing=True)
+geo = qd.geometry(16, 2, 64, {dtype})
+pool = torch.zeros(4 * qd.block_bytes(geo), dtype=torch.uint8, device="cuda")
+i = torch.zeros(1, dtype=torch.int32, device="cuda")
+q, out, x = torch.ones(1, 8, 64, device="cuda"), torch.full((1, 8, 64), 3.0, device="cuda"), torch.ones(1, 12 * 64, device="cuda")
+rows, back = torch.full((1, 256), 2.0, device="cuda"), torch.zeros(1, 256, device="cuda")
+torch.cuda.synchronize()
+side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=side):
+    s = side.cuda_stream
+    dev.kv_sync(geo, pool, rows, i, stream=s)
+    dev.kv_read(geo, pool, i, back, stream=s)
+    dev.head_prelude(geo, 8, x[:, :512], x[:, 512:640], x[:, 640:], i, q, stream=s)
+    dev.attn_decode_window(geo, pool, 8, q, i, i, i, 0, out, stream=s)
+g.replay()
+torch.cuda.synchronize()
+assert (back == 2).all() and (out == 2).all(), (back, out)
+dev.close()
+"""
+
+
+@pytest.mark.parametrize("dtype", ["BF16", "Q4"])
+def test_the_first_call_of_a_process_may_be_a_captured_one(dtype):
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE.format(dtype="qd." + dtype)], cwd=Path(__file__).resolve().parent.parent,
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

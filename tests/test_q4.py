@@ -221,3 +221,47 @@ def test_what_a_4_bit_pool_cannot_do_is_refused(dev):
         dev.check(dev.lib.qvx_kv_read(dev.h, C.byref(geo), buf.ptr, 4, t.data_ptr(), 1, x.data_ptr(), qd.Q4, None))
     assert dev.supports(qd.Q4) and not dev.supports(4)
     buf.free()
+
+
+@pytest.mark.gpu
+def test_a_misaligned_pool_is_refused(dev):
+    import torch
+    geo = qd.geometry(16, 1, 64, qd.Q4)
+    bb = qd.block_bytes(geo)
+    pool = torch.zeros(2 * bb + 16, dtype=torch.uint8, device="cuda")[2:2 + 2 * bb]
+    at, rows = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, 128, device="cuda")
+    for call in (lambda: dev.kv_sync(geo, pool, rows, at), lambda: dev.kv_append(geo, pool, rows[:, :64].contiguous(), rows[:, 64:].contiguous(), at, at, at),
+                 lambda: dev.kv_read(geo, pool, at, rows)):
+        with pytest.raises(qd.ShapeError):
+            call()
+
+
+@pytest.mark.gpu
+def test_a_runtime_over_a_4_bit_pool_shares_and_copies_blocks(dev):
+    """The runtime's own flow (plans, sync rows, prefix sharing, copy-on-write) with nothing changed but the element type."""
+    from plain import window_attention
+    from qubivex_b200.ondevice import AttnSeq, OnDevice
+
+    heads, kvh, d, prompt, steps = 8, 2, 64, 21, 14
+    geo = qd.geometry(16, kvh, d, qd.Q4)
+    od = OnDevice(dev, geo, heads, blocks=24)
+    rng = np.random.default_rng(6)
+    seqs = [AttnSeq(None, rng.standard_normal((kvh, prompt + steps, d)).astype(np.float32),
+                    rng.standard_normal((kvh, prompt + steps, d)).astype(np.float32), 0) for _ in range(3)]
+    seqs[1].host_k[:, :prompt], seqs[1].host_v[:, :prompt] = seqs[0].host_k[:, :prompt], seqs[0].host_v[:, :prompt]
+    for i in range(steps):
+        if i == 1:  # sequence 1 takes sequence 0's prompt as it lies in the pool
+            seqs[1].mirror.drop()
+            seqs[1].mirror = seqs[0].mirror.fork(prompt)
+        for s in seqs:
+            s.pos = prompt + i
+        q = rng.standard_normal((3, heads, d)).astype(np.float32)
+        k = np.stack([s.host_k[:, s.pos].reshape(-1) for s in seqs])
+        v = np.stack([s.host_v[:, s.pos].reshape(-1) for s in seqs])
+        out = od.attention(seqs, 0, q, k, v)
+        for t, s in enumerate(seqs):
+            kk, vv = (stands_for(x[:, : s.pos + 1].transpose(1, 0, 2), "q4") for x in (s.host_k, s.host_v))
+            want = window_attention(q[t], kk, vv, 0, 0)
+            assert np.linalg.norm(out[t] - want) <= 1e-5 * np.linalg.norm(want), (i, t)
+    assert od.kv.stats().cow_copies >= 1
+    od.close()
