@@ -2,7 +2,8 @@
 //
 // Store: a thread takes eight consecutive elements of a row; four neighbouring lanes hold a group of 32, find its least
 // and greatest value by shuffles, and each writes its eight codes; the first of the four writes the group's step and
-// offset.  Every store is the group's own bytes, so rows of one tile may be written by any blocks in any order.
+// offset.  Every store is the group's own bytes, so rows of one tile may be written by any blocks in any order.  16383 rows
+// of 8 x 128: about 36 us for 155 MB, bound by instructions (some 130 per 256 elements) before HBM.
 // Bound by HBM: 4 + 5/8 bytes per element.
 //
 // Read: a thread takes eight consecutive elements (one word of codes, or two half words) and writes them in the type
@@ -30,11 +31,11 @@ struct Q4RowArgs {
 };
 
 // A warp keeps to one piece of 256 consecutive elements of the rows (`n_row` such pieces to a row, eight elements a lane)
-// and goes through them Q4_ROWS at a time, the next ones on their way while these are worked on; the grid is what the
-// device holds at once.
-constexpr uint32_t Q4_ROWS = 2;
-template <int D>
-__global__ void __launch_bounds__(256, 3) kv_rows_q4_kernel(Q4RowArgs a, uint32_t n_row, uint32_t lines) {
+// and goes through them ROWS at a time, the next ones on their way while these are worked on; the grid is what the device
+// holds at once.  Two rows at a time; one where there are too few to give every warp two (100 rows: 2.4 us less latency
+// for the store and the read together).
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256, 4) kv_rows_q4_kernel(Q4RowArgs a, uint32_t n_row, uint32_t lines) {
     constexpr uint32_t d8 = D / 8;
     const uint32_t lane = threadIdx.x & 31u, half_row = a.L.kvh * d8;
     const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), line = gw / n_row, w = (gw - line * n_row) * 32u + lane;
@@ -44,11 +45,11 @@ __global__ void __launch_bounds__(256, 3) kv_rows_q4_kernel(Q4RowArgs a, uint32_
     const float* const src = (kv ? a.v_rows : a.k_rows) + 8u * e;
     const Q4Place<D> place(kv, i);
     uint8_t* const at_head = a.pool + (uint64_t)g * 2u * a.L.page_bytes;
-    float next[Q4_ROWS][8];
-    uint32_t p_next[Q4_ROWS];
+    float next[ROWS][8];
+    uint32_t p_next[ROWS];
     auto fetch = [&](uint32_t r0) {
 #pragma unroll
-        for (uint32_t u = 0; u < Q4_ROWS; u++) {
+        for (int u = 0; u < ROWS; u++) {
             const uint32_t r = r0 + u;
             p_next[u] = QVX_POS_NONE;
 #pragma unroll
@@ -66,22 +67,22 @@ __global__ void __launch_bounds__(256, 3) kv_rows_q4_kernel(Q4RowArgs a, uint32_
             p_next[u] = a.at_direct ? a.at_direct[r] : a.pos[r];
         }
     };
-    fetch(line * Q4_ROWS);
-    for (uint32_t r0 = line * Q4_ROWS; r0 < a.n; r0 += lines * Q4_ROWS) {
-        float x[Q4_ROWS][8];
-        uint32_t block[Q4_ROWS], slot[Q4_ROWS];
-        bool store[Q4_ROWS];
+    fetch(line * ROWS);
+    for (uint32_t r0 = line * ROWS; r0 < a.n; r0 += lines * ROWS) {
+        float x[ROWS][8];
+        uint32_t block[ROWS], slot[ROWS];
+        bool store[ROWS];
 #pragma unroll
-        for (uint32_t u = 0; u < Q4_ROWS; u++) {
+        for (int u = 0; u < ROWS; u++) {
 #pragma unroll
             for (int k = 0; k < 8; k++) x[u][k] = next[u][k];
             store[u] = p_next[u] != QVX_POS_NONE;
             split_position(p_next[u], a.L.B, a.shift, block[u], slot[u]);
             if (store[u] && !a.at_direct) block[u] = a.blocks[a.table_at[r0 + u] + block[u]];
         }
-        if (r0 + lines * Q4_ROWS < a.n) fetch(r0 + lines * Q4_ROWS);
+        if (r0 + lines * ROWS < a.n) fetch(r0 + lines * ROWS);
 #pragma unroll
-        for (uint32_t u = 0; u < Q4_ROWS; u++) {
+        for (int u = 0; u < ROWS; u++) {
             __half step, offset;
             const uint32_t codes = q4_quantise(x[u], step, offset);
             if (store[u] && block[u] >= a.pool_blocks) { atomicExch(a.status, STATUS_BLOCK_OUT_OF_POOL); store[u] = false; }
@@ -96,18 +97,23 @@ int32_t launch_kv_rows_q4(qvx_device* dev, const Layout& L, void* pool, const fl
     if (n > 0x7fffffffu) return fail(dev, QVX_ERR_CORE, "kv rows: %zu rows do not fit 31 bits", n);
     if ((uintptr_t)pool & 15u) return fail(dev, QVX_ERR_SHAPE, "shape mismatch in kv rows: a 4-bit pool must be 16-byte aligned");
     const uint32_t n_row = (L.kvh * (L.d / 8) * 2u + 31u) / 32u;
-    // Lines of warps, one per piece of a row: as many as there are rows for, or as the device holds (24 warps an SM).
-    const uint64_t held = std::max<uint64_t>(1, 24ull * dev->prop.multiProcessorCount / n_row);
-    const uint32_t lines = (uint32_t)std::min<uint64_t>((n + Q4_ROWS - 1) / Q4_ROWS, held);
+    // Lines of warps, one per piece of a row: as many as there are rows for, or as the device holds (32 warps an SM).
+    const uint64_t held = std::max<uint64_t>(1, 32ull * dev->prop.multiProcessorCount / n_row);
+    const uint32_t each = n > held ? 2 : 1;
+    const uint32_t lines = (uint32_t)std::min<uint64_t>((n + each - 1) / each, held);
     const uint64_t grid = ((uint64_t)lines * n_row + 7) / 8;
     if (grid > 0x7fffffffull) return fail(dev, QVX_ERR_CORE, "kv rows: rows of %zu elements are too long for one launch", (size_t)L.kvh * L.d);
     const uintptr_t ends = (uintptr_t)k_rows | (uintptr_t)v_rows | (uintptr_t)(row_stride_f32 * 4);
     Q4RowArgs a{L, (uint8_t*)pool, k_rows, v_rows, row_stride_f32, at_direct, pos, blocks, table_at, (uint32_t)n,
                 (uint32_t)std::min<size_t>(pool_blocks, 0xffffffffu), block_shift(L.B), ends % 32 == 0 ? 32u : ends % 16 == 0 ? 16u : 0u, device_status_word(dev)};
     LaunchTimer timer(dev, kind, s);
-    if (L.d == 64) kv_rows_q4_kernel<64><<<(unsigned)grid, 256, 0, s>>>(a, n_row, lines);
-    else if (L.d == 128) kv_rows_q4_kernel<128><<<(unsigned)grid, 256, 0, s>>>(a, n_row, lines);
-    else kv_rows_q4_kernel<256><<<(unsigned)grid, 256, 0, s>>>(a, n_row, lines);
+#define QVX_ROWS(DD)                                                                                 \
+    if (L.d == DD && each == 1) kv_rows_q4_kernel<DD, 1><<<(unsigned)grid, 256, 0, s>>>(a, n_row, lines); \
+    if (L.d == DD && each == 2) kv_rows_q4_kernel<DD, 2><<<(unsigned)grid, 256, 0, s>>>(a, n_row, lines);
+    QVX_ROWS(64)
+    QVX_ROWS(128)
+    QVX_ROWS(256)
+#undef QVX_ROWS
     return check_cuda(dev, cudaGetLastError(), "4-bit kv rows launch");
 }
 
@@ -169,23 +175,23 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     }
 }
 
-// 4-bit pools: a warp takes 256 consecutive elements of READ_ROWS consecutive rows (n_row: such pieces of a row).
-constexpr uint32_t READ_ROWS = 4;
-template <int D>
+// 4-bit pools: a warp takes 256 consecutive elements of ROWS consecutive rows (n_row: such pieces of a row): four, or one
+// where there are too few rows.
+template <int D, int ROWS>
 __global__ void __launch_bounds__(256) kv_read_q4_kernel(ReadArgs a, uint32_t n_row) {
     constexpr uint32_t d8 = D / 8;
     const uint32_t lane = threadIdx.x & 31u, half_row = a.L.kvh * d8;
-    const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), r0 = gw / n_row * READ_ROWS, w = gw % n_row * 32u + lane;
+    const uint32_t gw = blockIdx.x * 8u + (threadIdx.x >> 5), r0 = gw / n_row * ROWS, w = gw % n_row * 32u + lane;
     if (r0 >= a.n || w >= 2u * half_row) return;
     const uint32_t kv = w >= half_row ? 1u : 0u, e = w - kv * half_row, g = e / d8;
     const Q4Place<D> place(kv, e % d8 * 8u);
     const uint8_t* const at_head = a.pool + (uint64_t)g * 2u * a.L.page_bytes;
-    uint32_t p[READ_ROWS], c[READ_ROWS];
-    __half step[READ_ROWS], off[READ_ROWS];
+    uint32_t p[ROWS], c[ROWS];
+    __half step[ROWS], off[ROWS];
 #pragma unroll
-    for (uint32_t u = 0; u < READ_ROWS; u++) p[u] = r0 + u < a.n ? a.from[r0 + u] : QVX_POS_NONE;
+    for (int u = 0; u < ROWS; u++) p[u] = r0 + u < a.n ? a.from[r0 + u] : QVX_POS_NONE;
 #pragma unroll
-    for (uint32_t u = 0; u < READ_ROWS; u++) {
+    for (int u = 0; u < ROWS; u++) {
         if (p[u] == QVX_POS_NONE) continue;
         uint32_t block, slot;
         split_position(p[u], a.L.B, a.shift, block, slot);
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(256) kv_read_q4_kernel(ReadArgs a, uint32_t n_
         off[u] = *reinterpret_cast<const __half*>(tile + place.offset_at(slot));
     }
 #pragma unroll
-    for (uint32_t u = 0; u < READ_ROWS; u++) {
+    for (int u = 0; u < ROWS; u++) {
         if (p[u] == QVX_POS_NONE) continue;
         // A code in bits 0..3 of a half word is the f16 number c 2^-24, in bits 4..7 c 2^-20: converting those is exact.
         const float z = __half2float(off[u]), s0 = __half2float(step[u]) * 16777216.f, s1 = s0 * 0.0625f;
@@ -245,13 +251,18 @@ int32_t launch_kv_read(qvx_device* dev, const Layout& L, const void* pool, size_
                      (uintptr_t)rows % 32 == 0 ? 32u : (uintptr_t)rows % 16 == 0 ? 16u : 0u, device_status_word(dev)};
     if (L.dtype == QVX_Q4) {
         const uint32_t n_row = (L.kvh * (L.d / 8) * 2u + 31u) / 32u;
-        const uint64_t warps = (uint64_t)((n + READ_ROWS - 1) / READ_ROWS) * n_row;
+        const uint32_t each = (uint64_t)n * n_row > 32ull * dev->prop.multiProcessorCount ? 4 : 1;
+        const uint64_t warps = (uint64_t)((n + each - 1) / each) * n_row;
         if (warps > 0x7fffffffull) return fail(dev, QVX_ERR_CORE, "kv read: %zu rows are too many for one launch", n);
         const unsigned grid = (unsigned)((warps + 7) / 8);
         LaunchTimer timer(dev, QVX_K_COPY, s);
-        if (L.d == 64) kv_read_q4_kernel<64><<<grid, 256, 0, s>>>(a, n_row);
-        else if (L.d == 128) kv_read_q4_kernel<128><<<grid, 256, 0, s>>>(a, n_row);
-        else kv_read_q4_kernel<256><<<grid, 256, 0, s>>>(a, n_row);
+#define QVX_READ(DD)                                                                     \
+    if (L.d == DD && each == 1) kv_read_q4_kernel<DD, 1><<<grid, 256, 0, s>>>(a, n_row); \
+    if (L.d == DD && each == 4) kv_read_q4_kernel<DD, 4><<<grid, 256, 0, s>>>(a, n_row);
+        QVX_READ(64)
+        QVX_READ(128)
+        QVX_READ(256)
+#undef QVX_READ
         return check_cuda(dev, cudaGetLastError(), "4-bit kv read launch");
     }
     const uint32_t width = L.d % 8 == 0 ? 8 : 1;
