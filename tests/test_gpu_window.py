@@ -356,3 +356,27 @@ def test_the_first_call_of_a_process_may_be_a_captured_one(dtype):
     r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE.format(dtype="qd." + dtype)], cwd=Path(__file__).resolve().parent.parent,
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype,spare", [("bf16", 150000), ("q4", 480000), ("f32", 75000)])
+def test_pools_past_four_gibibytes(dev, dtype, spare):
+    """Blocks scattered over a pool whose byte offsets pass 32 bits: stored, read back and attended over."""
+    b = Batch(dev, [700, 33], 8, 4, 128, 16, dtype, spare=spare)
+    assert b.pool.numel() > 1 << 32 and int(b.blocks.max()) * qd.block_bytes(b.geo) > 1 << 32
+    b.check(b.run())
+    p = np.arange(700)
+    at = b.torch.from_numpy((b.blocks[p // 16].astype(np.int64) * 16 + p % 16).astype(np.int32)).cuda()
+    got = dev.kv_read(b.geo, b.pool, at, b.torch.empty(700, 2 * 4 * 128, device="cuda"))
+    assert np.array_equal(got.cpu().numpy(), stands_for(b.rows[0].reshape(700, -1), dtype).astype(np.float32))
+
+
+def test_a_pool_of_the_devices_own(dev):
+    """A DeviceBuffer in place of a tensor."""
+    b = Batch(dev, [100, 9], 8, 2, 64, 16, "q4")
+    buf = dev.alloc(b.pool.numel())
+    dev.write(buf, 0, b.pool.cpu().numpy())
+    tensor, want = b.pool, b.run()
+    b.pool = buf
+    assert b.torch.equal(b.run(), want)
+    b.pool = tensor
+    buf.free()
