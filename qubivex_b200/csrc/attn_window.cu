@@ -815,8 +815,11 @@ struct WindowKernel {
     uint32_t held[17] = {};
 };
 
+// `ranks` CTAs per cluster of a launch of `units` clusters: as many as leave every cluster resident at once (64 long 4-bit
+// sequences: 107 us with clusters of 6, 115 with 4, 134 with 8, which come in two waves) and every second warp at least in
+// work (4 x 37-512 positions: 4.4 us with half of 8 CTAs' warps idle, 5.0 with 4 CTAs).  With go: the launch as well.
 template <class T, int D, int NW, int STAGES, int MIN_CTAS>
-static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, int ordinal, dim3 grid, cudaStream_t s) {
+static cudaError_t window_ranks(const WindowArgs& a, uint64_t units, uint32_t tiles, int ordinal, uint32_t& ranks, bool go, dim3 grid, cudaStream_t s) {
     auto* kernel = attn_window_kernel<T, D, NW, STAGES, MIN_CTAS>;
     using SM = WindowSmem<T, D, NW, STAGES>;
     cudaLaunchConfig_t cfg{};
@@ -844,19 +847,30 @@ static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t t
             k.ready = true;
         }
     }
-    // CTAs per cluster: as many as leave every cluster resident at once and every warp in work.  (64 long 4-bit sequences:
-    // 107 us with clusters of 6, 115 with 4, 134 with 8, which come in two waves.)
-    uint32_t ranks = 1;
+    ranks = 1;
     for (uint32_t r = 2; r <= 16; r = r < 8 ? r + 1 : r + 8)
-        if (units <= k.held[r] && r * NW * T::SUB <= tiles) ranks = r;
+        if (units <= k.held[r] && r * NW <= 2 * tiles) ranks = r;
 #ifdef QVX_EXPERIMENTS
     if (const char* v = getenv("QVX_WINDOW_RANKS")) ranks = (uint32_t)atol(v);
 #endif
+    if (!go) return cudaSuccess;
     grid.x = ranks;
     cfg.gridDim = grid;
     cfg.stream = s;
     at[0].val.clusterDim.x = ranks;
     return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// CTAs of four warps; of eight where four would leave one CTA to an SM at most and every warp a few stages of work.
+template <class T, int D, int STAGES, int MIN_CTAS, bool EIGHT>
+static cudaError_t launch_window(const WindowArgs& a, uint64_t units, uint32_t tiles, uint32_t sms, int ordinal, dim3 grid, cudaStream_t s) {
+    uint32_t ranks = 1;
+    if constexpr (EIGHT) {
+        cudaError_t e = window_ranks<T, D, 4, STAGES, MIN_CTAS>(a, units, tiles, ordinal, ranks, false, grid, s);
+        if (e != cudaSuccess) return e;
+        if (units * ranks <= sms && tiles >= ranks * 8 * T::SUB * 2) return window_ranks<T, D, 8, STAGES, 1>(a, units, tiles, ordinal, ranks, true, grid, s);
+    }
+    return window_ranks<T, D, 4, STAGES, MIN_CTAS>(a, units, tiles, ordinal, ranks, true, grid, s);
 }
 
 int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, size_t pool_blocks, size_t heads, size_t s, const float* q,
@@ -884,21 +898,22 @@ int32_t launch_attn_window(qvx_device* dev, const Layout& L, const void* pool, s
     const uint64_t units = (uint64_t)grid.y * grid.z;
     LaunchTimer timer(dev, QVX_K_ATTN, stream);
     cudaError_t e = cudaErrorInvalidValue;
-#define QVX_WINDOW(TYPE, TILE_T, DD, STG, CTAS) \
-    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, 4, STG, CTAS>(a, units, tiles, dev->ordinal, grid, stream);
+    const uint32_t sms = (uint32_t)dev->prop.multiProcessorCount;
+#define QVX_WINDOW(TYPE, TILE_T, DD, STG, CTAS, EIGHT) \
+    if (L.dtype == TYPE && L.d == DD) e = launch_window<TILE_T, DD, STG, CTAS, EIGHT>(a, units, tiles, sms, dev->ordinal, grid, stream);
 #define QVX_COMMA ,
-    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 64>, 64, 3, 4)
-    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 128>, 128, 3, 2)
-    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 256>, 256, 3, 1)
-    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 64>, 64, 3, 4)
-    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 128>, 128, 3, 2)
-    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 256>, 256, 3, 1)
-    QVX_WINDOW(QVX_F32, Tile32<64>, 64, 3, 4)
-    QVX_WINDOW(QVX_F32, Tile32<128>, 128, 3, 2)
-    QVX_WINDOW(QVX_F32, Tile32<256>, 256, 3, 1)
-    QVX_WINDOW(QVX_Q4, TileQ4<64>, 64, 2, 4)
-    QVX_WINDOW(QVX_Q4, TileQ4<128>, 128, 2, 3)
-    QVX_WINDOW(QVX_Q4, TileQ4<256>, 256, 2, 2)
+    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 64>, 64, 3, 4, true)
+    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 128>, 128, 3, 2, true)
+    QVX_WINDOW(QVX_BF16, Tile16<QVX_BF16 QVX_COMMA 256>, 256, 3, 1, false)  // (eight warps' rings do not fit)
+    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 64>, 64, 3, 4, true)
+    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 128>, 128, 3, 2, true)
+    QVX_WINDOW(QVX_F16, Tile16<QVX_F16 QVX_COMMA 256>, 256, 3, 1, false)
+    QVX_WINDOW(QVX_F32, Tile32<64>, 64, 3, 4, true)
+    QVX_WINDOW(QVX_F32, Tile32<128>, 128, 3, 2, true)
+    QVX_WINDOW(QVX_F32, Tile32<256>, 256, 3, 1, false)
+    QVX_WINDOW(QVX_Q4, TileQ4<64>, 64, 2, 4, true)
+    QVX_WINDOW(QVX_Q4, TileQ4<128>, 128, 2, 3, true)
+    QVX_WINDOW(QVX_Q4, TileQ4<256>, 256, 2, 2, true)
 #undef QVX_COMMA
 #undef QVX_WINDOW
     return check_cuda(dev, e, "window attention launch");

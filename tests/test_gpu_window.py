@@ -111,6 +111,15 @@ def test_long_contexts(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "q4"])
+@pytest.mark.parametrize("d,heads,kvh", [(64, 8, 1), (64, 3, 1), (128, 6, 2), (256, 8, 1)])
+def test_one_long_sequence_alone(dev, dtype, d, heads, kvh):
+    """Few clusters, each with all the CTAs and warps there are."""
+    b = Batch(dev, [7001], heads, kvh, d, 16, dtype, seed=d)
+    b.check(b.run())
+    b.check(b.run(3000, 33), 3000, 33)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16", "q4"])
 def test_large_and_small_numbers(dev, dtype):
     """Scores of a few hundred (one position takes everything), values of very different size, queries that f16 alone could
     not hold; the steps of a 4-bit pool's values grow and shrink along the sequence."""
