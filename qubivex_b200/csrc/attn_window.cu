@@ -14,13 +14,13 @@
 // 308 us, 99 %; bf16, 64 sequences, 32 over 4 of 128, window 1024: 26 us, 80 %; 4 bits, 16 x 32768 positions, 32 over 4 of
 // 128: 107 us, 48 %; 4 bits, 64 x 1024-4096 positions: 54 us, 30 %.
 //
-// Data path.  Every warp has a ring of tiles of its own that its first lane fills with bulk copies, completion on
+// Data path.  Every warp has a ring of tiles of its own that its lanes fill in turn with bulk copies, completion on
 // mbarriers; nobody waits for another warp until the states are joined.
 //
 // Arithmetic.  Scores S = Q K^T by mma.sync with the queries as A (8 heads padded to 16 rows: rows 0..7 hold the value
 // rounded to the operand type, rows 8..15 the remainder, so one instruction carries both) and the keys as B.  A lane
 // then holds head lane / 4 at positions 2 (lane & 3), +1 (and +8, +9), which is how B of O^T = V^T P^T wants the
-// probabilities: they go in as value and remainder, in two passes, with no transposition.
+// probabilities: they go in as value and remainder, in two passes, with no transposition.  (bf16: a third part of both.)
 #include <stdlib.h>
 
 #include <algorithm>

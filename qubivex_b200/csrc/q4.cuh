@@ -28,22 +28,13 @@ namespace qvx {
 QVX_HD uint32_t q4_row(uint32_t r) { return (r & 8u) | ((r & 1u) << 2) | ((r >> 1) & 3u); }
 QVX_HD uint32_t q4_swap(uint32_t d, uint32_t row) { return d == 128 ? ((row >> 1) & 1u) << 2 : d == 256 ? (row & 3u) << 1 : 0u; }
 
-// Byte offsets in a tile of slot r (0..15): the 16-bit half holding codes of dimensions 4 j .. 4 j + 3, and the step
-// and the offset of group `grp`.
+// Byte offset in a tile of the 16-bit half that holds slot r's codes of dimensions 4 j .. 4 j + 3.
 QVX_HD uint32_t q4_codes_at(uint32_t d, uint32_t r, uint32_t kv, uint32_t j) {
     const uint32_t ng = d / Q4_GROUP, grp = j >> 3, u = j & 7u;
     if (!kv) return r * (d / 2) + ((u >> 1) * ng + grp) * 4 + (u & 1u) * 2;
     const uint32_t row = q4_row(r);
     return 8 * d + row * (d / 2) + ((u ^ q4_swap(d, row)) * ng + grp) * 2;
 }
-QVX_HD uint32_t q4_step_at(uint32_t d, uint32_t r, uint32_t kv, uint32_t grp) {
-    return (kv ? 17 : 16) * d + ((r >> 1) * (d / Q4_GROUP) + grp) * 4 + (r & 1u) * 2;
-}
-QVX_HD uint32_t q4_offset_at(uint32_t d, uint32_t r, uint32_t kv, uint32_t grp) {
-    const uint32_t ng = d / Q4_GROUP;
-    return kv ? 19 * d + ((r >> 1) * ng + grp) * 4 + (r & 1u) * 2 : 18 * d + (r * ng + grp) * 2;
-}
-
 #if defined(__CUDACC__)
 // Four neighbouring lanes hold a group, eight elements each.  All 32 lanes call it.  Gives the lane's eight codes (code n
 // in bits 4 n .. 4 n + 3) and the group's step and offset.
